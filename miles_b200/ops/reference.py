@@ -278,6 +278,24 @@ def fp8_block128_quant(x: torch.Tensor, ue8m0: bool = False):
     return q, s
 
 
+def fp8_block128_dequant(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    """fp32 values of ``[..., rows, cols]`` E4M3 numbers with a scale for each 128 x 128."""
+    wide = s.repeat_interleave(128, -2)[..., :q.shape[-2], :].repeat_interleave(128, -1)[..., :q.shape[-1]]
+    return q.float() * wide
+
+
+def fp8_rows_quant(x: torch.Tensor):
+    """8-bit rows: E4M3 values of ``x [T, K]`` and an fp32 scale for each row and 128 columns, ``max(amax, 1e-10) / 448``."""
+    xp = F.pad(x.float(), (0, (-x.shape[1]) % 128))
+    s = xp.reshape(x.shape[0], xp.shape[1] // 128, 128).abs().amax(-1).clamp_min(1e-10) / 448.0
+    q = (x.float() / s.repeat_interleave(128, -1)[:, :x.shape[1]]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return q, s
+
+
+def fp8_rows_dequant(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    return q.float() * s.repeat_interleave(128, -1)[:, :q.shape[1]]
+
+
 def fake_int4_quant(x: torch.Tensor, gr: int, gc: int, sym: bool):
     rows, cols = x.shape
     xf = x.float().reshape(rows // gr, gr, cols // gc, gc).permute(0, 2, 1, 3)
