@@ -24,7 +24,9 @@ struct Fp8Gemm {
   uint8_t* q;         // gated: silu(gate) * up as 8-bit rows [M, N / 2] ...
   float* s;           // ... and their scales [M, ceil(N / 2 / 128)]
   int* status;        // device status word (0 = ok), may be null
+  void* workspace;    // fp8_gemm_workspace bytes, 16-byte aligned
 };
+long long fp8_gemm_workspace(const Fp8Gemm& p);
 // Launches on `stream`. Returns 0 or -1 with the reason in fp8_last_error().
 int fp8_gemm_launch(const Fp8Gemm& p, cudaStream_t stream);
 const char* fp8_last_error();

@@ -3,14 +3,19 @@
 //   y[t, n] = (residual[t, n] +) sum over blocks b of 128 along K of  xs[t, b] ws[n / 128, b] sum over k in b of x[t, k] w[n, k]
 //
 // in E4M3 with fp32 scales of any value, so that no scale can ride in the tensor core's own (power-of-two) ones: a block's product is
-// computed by four tcgen05.mma into a TMEM buffer of its own, and eight warps add it, scaled, to sums in registers while the tensor core
-// fills the next buffer. Per 128 x 256 x 128 block the tensor core needs 512 clocks, the warps about 256 multiply-adds per scheduler.
-// The rows are one batch, or sorted by expert (row tiles {matrix, first row, rows} as the router's sort leaves them). A gate-up weight's
-// tile takes 128 gate rows and their 128 up rows, so that silu(gate) * up leaves as a whole block of 128 columns of 8-bit rows, scaled by
-// their largest value, without passing through memory in between.
+// computed by four tcgen05.mma into a TMEM buffer of its own, and warps add it, scaled, to sums in registers while the tensor core fills the
+// next buffers. The rows are one batch, or sorted by expert (row tiles {matrix, first row, rows} as the router's sort leaves them). A gate-up
+// weight's tile takes 128 gate rows and their 128 up rows, so that silu(gate) * up leaves as a whole block of 128 columns of 8-bit rows,
+// scaled by their largest value, without passing through memory in between.
 //
-//   warp 0     : TMA producer (128-byte swizzle)          warp 1 : TMEM allocator, tcgen05.mma issuer
-//   warps 2..9 : sums of a tile in registers (two warps per 32 rows, half of the columns each), then rows of 64 bytes through shared memory
+// A pair of CTAs (`cta_group::2`) computes 256 rows x 256 columns, each CTA its 128 rows, as two products of 128 columns a block. Four of
+// those fit TMEM. That many are needed: about 630 clocks pass from the end of a product to the start of the one that may overwrite it even
+// if nobody reads it, and a reader's loads and multiply-adds take 250 more, so that two buffers of 256 columns (one CTA) leave the tensor core
+// idle for a third of the time, while four of 128 take 4 x 256 clocks to come round. One CTA alone cannot use four: its products of 128
+// columns take 417 clocks a block instead of 256.
+//
+//   warp 0      : TMA producer (128-byte swizzle)          warps 1, 2 : tcgen05.mma issuers (1 allocates TMEM)          (3: none)
+//   warps 4..11 : sums in registers, a row and 64 columns of each half a thread, then rows of 128 bytes through shared memory
 //
 // Reference counterpart: the block-wise FP8 GEMMs of the serving engines that load its FP8 checkpoints (weight_block_size [128, 128]:
 // miles/backends/megatron_utils/megatron_to_hf/processors/quantizer_fp8.py, miles/utils/fp8_kernel.py:24-79).
@@ -20,6 +25,7 @@
 #include <atomic>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "fp8_block.h"
 #include "fp8_math.cuh"
@@ -28,11 +34,13 @@
 namespace mb {
 namespace {
 
-constexpr int BM = 128, BK = 128;
-constexpr int HALF_BYTES = 128 * BK;  // 128 rows of one operand and stage
-constexpr int THREADS = 320;
-constexpr int EPI_WARPS = 8;
-constexpr int STAGING = EPI_WARPS * 4096;
+constexpr int BM = 128, BN = 256, BK = 128;  // rows of a CTA, columns of its pair's tile (W rows), columns of a block
+constexpr int COLS = 128;                    // of a tile's half: a thread's
+constexpr int STAGES = 6, BUFS = 4;          // (an even number of stages: each issuer has its own)
+constexpr int X_BYTES = BM * BK, W_HALF_BYTES = 64 * BK;  // of a stage: this CTA's rows of x; its 64 W rows of each half
+constexpr int STAGE = X_BYTES + 2 * W_HALF_BYTES;
+constexpr int THREADS = 384;                 // three warpgroups: the second and third sum up, with registers that the first gives back
+constexpr int STAGING = 8 * 4096;
 
 struct Args {
   int M, N, K;
@@ -40,28 +48,34 @@ struct Args {
   const float* xs;
   const float* ws;
   int groups, max_tiles;
-  const int* tile_group;
+  const int4* tiles;               // {matrix, first row, rows, 0}: at most 256 rows each
   const int* num_tiles;
   __nv_bfloat16* y;
   long long ldy;
   const __nv_bfloat16* residual;
   long long ldr;
-  int vec_ok;
+  int vec_y, vec_r;                // 16-byte accesses fit
   uint8_t* q;
   float* s;
   int* status;
 };
 
+// An arrival that publishes no memory: a TMEM buffer is handed back, whose loads are complete and ordered by the fence before. (With
+// .release.cluster the second CTA's arrival waits 1200 to 1900 clocks for the thread's other accesses.)
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 struct Tile {
   int row0, row_end, n0, group;  // rows of x; first column of y (or of silu(gate) * up)
 };
 
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
       "}\n"
       :
       : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
@@ -73,61 +87,62 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
 }
 
 // The wait of a load from TMEM names its registers, so that nothing that reads them moves ahead of it while the next load is under way.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                 "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
                :
                : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
-
 // Whether every thread of the warp came out of its wait: the loads from TMEM behind it are the whole warp's.
 __device__ __forceinline__ bool all_got(bool got) { return __all_sync(0xffffffffu, got); }
 
-// Columns of a tile: BN of y, or BN / 2 of silu(gate) * up.
-template <int BN, bool GATED>
+template <bool GATED>
 __device__ __forceinline__ int column_tiles(const Args& p) {
-  constexpr int COLS = GATED ? BN / 2 : BN;
-  return (p.N / p.halves + COLS - 1) / COLS;
+  constexpr int W = GATED ? BN / 2 : BN;
+  return (p.N / p.halves + W - 1) / W;
 }
-template <int BN, bool GATED>
+template <bool GATED>
 __device__ __forceinline__ int tiles_of(const Args& p) {
-  int m = (p.M + BM - 1) / BM;
-  if (p.tile_group) m = min(max(*p.num_tiles, 0), p.max_tiles);
-  return m * column_tiles<BN, GATED>(p);
+  const int m = p.tiles ? min(max(*p.num_tiles, 0), p.max_tiles) : (p.M + 2 * BM - 1) / (2 * BM);
+  return m * column_tiles<GATED>(p);
 }
-template <int BN, bool GATED>
+template <bool GATED>
 __device__ __forceinline__ Tile tile_at(const Args& p, int t) {
-  const int n_tiles = column_tiles<BN, GATED>(p);
+  const int n_tiles = column_tiles<GATED>(p);
   Tile r;
   int mt = t / n_tiles, nt = t - mt * n_tiles;
-  if (p.tile_group) {
-    const int4 e = reinterpret_cast<const int4*>(p.tile_group)[mt];
-    r.group = min(max(e.x, 0), p.groups - 1);
-    r.row0 = min(max(e.y, 0), p.M);
-    r.row_end = min(p.M, r.row0 + min(max(e.z, 0), BM));
+  if (p.tiles) {
+    const int4 e = p.tiles[mt];
+    r.group = e.x;
+    r.row0 = e.y;
+    r.row_end = e.y + e.z;
   } else {
-    // bands of eight row tiles, their columns outermost: CTAs that run together share tiles of W in L2
-    constexpr int BAND = 8;
-    const int m_tiles = (p.M + BM - 1) / BM;
+    // bands of four row tiles, their columns outermost: pairs that run together share tiles of W in L2
+    constexpr int BAND = 4;
+    const int m_tiles = (p.M + 2 * BM - 1) / (2 * BM);
     const int band = t / (BAND * n_tiles), first = band * BAND;
     const int rows = min(m_tiles - first, BAND), in_band = t - band * BAND * n_tiles;
     mt = first + in_band % rows;
     nt = in_band / rows;
     r.group = 0;
-    r.row0 = mt * BM;
-    r.row_end = min(p.M, r.row0 + BM);
+    r.row0 = mt * 2 * BM;
+    r.row_end = min(p.M, r.row0 + 2 * BM);
   }
   r.n0 = nt * (GATED ? BN / 2 : BN);
   return r;
 }
 
-template <int BN, bool GATED, int STAGES>
+// What a thread multiplies its sums' blocks with: the scales of its row, and of the weights' block(s) that its columns are in.
+struct Scales {
+  const float *x, *w0, *w1;
+};
+
+template <bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args p) {
-  constexpr int BUFS = 512 / BN;                        // TMEM holds this many blocks' products
-  constexpr int STAGE = (BM + BN) * BK;
-  constexpr int COLS = BN / 2;                          // of the tile, per thread
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = base + STAGES * STAGE;
@@ -136,12 +151,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
   const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };                            // of the CTA of rank 0: both CTAs' copies have landed
   auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
-  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + BUFS + b); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + BUFS + b); };    // of the CTA of rank 0: both CTAs have read the buffer
   const uint32_t amax_bar = bar0 + 8u * (2 * STAGES + 2 * BUFS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int first_tile = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     abort_s = 0;
@@ -151,147 +168,193 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
     for (int b = 0; b < BUFS; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), EPI_WARPS);
+      mbar_init(tempty_bar(b), 16);  // eight warps of each CTA
     }
-    mbar_init(amax_bar, EPI_WARPS * 32);
+    mbar_init(amax_bar, 256);
     fence_barrier_init();
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_slot_s), 512);
-    tmem_relinquish();
-  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot_s), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot_s);
-  const int total = tiles_of<BN, GATED>(p);
+  cluster_sync_all();  // both CTAs' barriers and TMEM are there before either uses the other's
+  const int total = tiles_of<GATED>(p);
   const int half_n = p.N / p.halves;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const Tile tl = tile_at<BN, GATED>(p, t);
-        const int w0 = tl.group * p.N + tl.n0;
-        const int w1 = GATED ? w0 + half_n : w0 + 128;  // the tile's second 128 rows of W
-        for (int kb = 0; kb < p.blocks_k; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, ERR_WAIT_EMPTY)) {
-            ok = false;
-            break;
+  // 4 x 32 x 56 + 8 x 32 x 224 registers are the 384 x 168 of the launch
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (elect_one()) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = first_tile; ok && t < total; t += step) {
+          const Tile tl = tile_at<GATED>(p, t);
+          const int w0 = tl.group * p.N + tl.n0 + rank * 64;  // this CTA's rows of W: 64 of each half of the tile
+          const int w1 = w0 + (GATED ? half_n : 128);
+          for (int kb = 0; kb < p.blocks_k; ++kb) {
+            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, ERR_WAIT_EMPTY)) {
+              ok = false;
+              break;
+            }
+            if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * STAGE);
+            const uint32_t full = map_to_rank(full_bar(stage), 0), dst = base + stage * STAGE;
+            tma_load_2d_pair(dst, &map_x, full, kb * BK, tl.row0 + rank * BM);
+            tma_load_2d_pair(dst + X_BYTES, &map_w, full, kb * BK, w0);
+            tma_load_2d_pair(dst + X_BYTES + W_HALF_BYTES, &map_w, full, kb * BK, w1);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          const uint32_t dst = base + stage * STAGE;
-          mbar_expect_tx(full_bar(stage), STAGE);
-          tma_load_2d(dst, &map_x, full_bar(stage), kb * BK, tl.row0);
-          tma_load_2d(dst + HALF_BYTES, &map_w, full_bar(stage), kb * BK, w0);
-          if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &map_w, full_bar(stage), kb * BK, w1);
+        }
+        for (int s = 0; ok && s < STAGES; ++s) {  // the other CTA's commits have arrived before this one leaves
+          ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, ERR_WAIT_EMPTY);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-      }
-      if (!ok) {  // copies in flight get a bounded time to land before shared memory is released
-        const unsigned long long t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 2000000ull) {
+        if (!ok) {  // copies in flight get a bounded time to land before shared memory is released
+          const unsigned long long t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 2000000ull) {
+          }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    constexpr uint32_t idesc = idesc_e4m3(BM, BN);
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, tphase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-      for (int kb = 0; kb < p.blocks_k; ++kb) {
-        ok = all_got(mbar_wait(tempty_bar(buf), tphase ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY) &&
-                     mbar_wait(full_bar(stage), phase, abort_flag, p.status, ERR_WAIT_FULL));
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t x = base + stage * STAGE, w = x + HALF_BYTES;
+      __syncwarp();
+    } else if (warp <= 2) {
+      // Two issuers, by turns of the blocks. One is not enough: it cannot prepare a block while the products it has issued still read their
+      // descriptors, so its waits would leave the tensor core idle between blocks. (elect.sync tells the compiler that one thread
+      // issues: under `lane == 0` a block takes 1040 clocks instead of 512.)
+      if (rank == 0 && elect_one()) {
+        constexpr uint32_t idesc = idesc_e4m3(2 * BM, COLS);
+        const int turn = warp - 1;  // buffers 0 and 1, or 2 and 3; every second stage
+        const long long blocks = first_tile < total ? static_cast<long long>((total - 1 - first_tile) / step + 1) * p.blocks_k : 0;
+        int stage = turn;
+        uint32_t phase = 0, tphase = 0;
+        bool ok = true;
+        for (long long b = turn; ok && b < blocks; b += 2) {
+          ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, ERR_WAIT_FULL);
+          const uint32_t x = base + stage * STAGE;
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_f8(tmem + buf * BN, make_smem_desc(x + k * 32, 16, 1024), make_smem_desc(w + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
-          umma_commit(empty_bar(stage));
-          umma_commit(tfull_bar(buf));
-        }
-        __syncwarp();
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        if (++buf == BUFS) {
-          buf = 0;
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && mbar_wait(tempty_bar(2 * turn + h), tphase ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t w = x + X_BYTES + h * W_HALF_BYTES;
+#pragma unroll
+            for (int k = 0; k < BK / 32; ++k)
+              umma_f8_pair(tmem + (2 * turn + h) * COLS, make_smem_desc(x + k * 32, 16, 1024), make_smem_desc(w + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
+            umma_commit_pair(tfull_bar(2 * turn + h));
+          }
+          if (!ok) break;
+          umma_commit_pair(empty_bar(stage));
           tphase ^= 1u;
+          stage += 2;
+          if (stage >= STAGES) {
+            stage -= STAGES;
+            phase ^= 1u;
+          }
         }
       }
+      __syncwarp();
     }
   } else {
-    const int quad = warp & 3, side = (warp - 2) >> 2;  // rows of the tile that this warp reaches in TMEM; its half of the columns
-    const uint32_t mine = staging + (warp - 2) * 4096;
-    int buf = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int quad = warp & 3, side = (warp - 4) >> 2;  // rows of the tile that this warp reaches in TMEM; its 64 columns of each half
+    const uint32_t mine = staging + (warp - 4) * 4096;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const auto scales_of = [&](const Tile& tl) {
+      Scales r;
+      const int row = min(tl.row0 + rank * BM + quad * 32 + lane, p.M - 1);
+      const int nb = tl.n0 / 128;
+      r.x = p.xs + static_cast<long long>(row) * p.blocks_k;
+      r.w0 = p.ws + (static_cast<long long>(tl.group) * p.blocks_n + nb) * p.blocks_k;
+      r.w1 = r.w0 + static_cast<long long>(GATED ? p.blocks_n / 2 : nb + 1 < p.blocks_n ? 1 : 0) * p.blocks_k;
+      return r;
+    };
+    // Between blocks as few instructions as can be: the additions alone take half of the clocks that the products leave. So a wait that
+    // runs out is looked at once a tile (what is read meanwhile is thrown away, and every later wait ends at once), and a buffer is
+    // handed back by one lane without a word from the others: the wait for their loads is the whole warp's.
+    const uint32_t tempty0 = map_to_rank(tempty_bar(0), 0);
+    const auto release = [&](int buf) {
+      tc_fence_before();
+      if (lane == 0) arrive_relaxed(tempty0 + 8u * buf);
+    };
+    int turn = 0, tiles_done = 0;
     uint32_t tphase = 0;
-    int turn = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < total; t += gridDim.x, ++turn) {
-      const Tile tl = tile_at<BN, GATED>(p, t);
-      const int row = tl.row0 + quad * 32 + lane;
-      const float* xs = p.xs + static_cast<long long>(min(row, p.M - 1)) * p.blocks_k;
-      // scales of the weights' block(s) of this thread's columns: one for all, or the gate's and the up rows'
-      const int nb = min(tl.n0 / 128 + (!GATED && BN == 256 ? side : 0), p.blocks_n / p.halves - 1);
-      const float* ws0 = p.ws + (static_cast<long long>(tl.group) * p.blocks_n + nb) * p.blocks_k;
-      const float* ws1 = ws0 + (GATED ? static_cast<long long>(p.blocks_n / 2) * p.blocks_k : 0);
-      float acc[COLS];
+    float xn = 0.f, wn0 = 0.f, wn1 = 0.f;  // of the next block
+    Scales sc = {};
+    Tile tl = {};
+    if (first_tile < total) {
+      tl = tile_at<GATED>(p, first_tile);
+      sc = scales_of(tl);
+      xn = sc.x[0];
+      wn0 = sc.w0[0];
+      wn1 = sc.w1[0];
+    }
+    for (int t = first_tile; t < total; t += step, ++tiles_done) {
+      float acc[COLS];  // 64 columns of each half
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-      float xn = xs[0], wn0 = ws0[0], wn1 = GATED ? ws1[0] : 0.f;
-      for (int kb = 0; kb < p.blocks_k; ++kb) {
-        const float c0 = xn * wn0, c1 = GATED ? xn * wn1 : c0;
-        if (kb + 1 < p.blocks_k) {
-          xn = xs[kb + 1];
-          wn0 = ws0[kb + 1];
-          if (GATED) wn1 = ws1[kb + 1];
-        }
-        ok = all_got(mbar_wait(tfull_bar(buf), tphase, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
-        if (!ok) break;
+      // 32 columns are under way while 32 are added, from half to half and block to block. Both warps of a scheduler read a half
+      // together, so that it is handed back as soon as can be.
+      uint32_t d[2][32];
+      const auto begin = [&](int buf) {  // its first columns
+        ok = mbar_wait(tfull_bar(buf), tphase, abort_flag, p.status, ERR_WAIT_TMEM_FULL) && ok;
+        __syncwarp();
         tc_fence_after();
-        // thread's columns: COLS from side * COLS on, or (gated) COLS / 2 gate columns and the same up columns
-        const uint32_t from = tmem + buf * BN + (static_cast<uint32_t>(quad * 32) << 16);
-        const auto col = [&](int c) {
-          return static_cast<uint32_t>(GATED ? (c < COLS / 2 ? side * (COLS / 2) + c : BN / 2 + side * (COLS / 2) + c - COLS / 2) : side * COLS + c);
-        };
-        uint32_t d[2][16];
-        tmem_ld_32x16(from + col(0), d[0]);
+        tmem_ld_32x32(tmem + buf * COLS + side * 64 + lanes, d[0]);
+      };
+      const auto add = [&](int at, float c, const uint32_t(&v)[32]) {
 #pragma unroll
-        for (int c = 0; c < COLS; c += 16) {
-          const int now = (c / 16) & 1;
-          tmem_ld_wait_for(d[now]);
-          if (c + 16 < COLS) {
-            tmem_ld_32x16(from + col(c + 16), d[now ^ 1]);
-          } else {  // everything has left the buffer
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty_bar(buf));
-          }
-          const float cc = GATED && c >= COLS / 2 ? c1 : c0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(cc, __uint_as_float(d[now][i]), acc[c + i]);
-        }
-        if (++buf == BUFS) {
-          buf = 0;
+        for (int i = 0; i < 32; ++i) acc[at + i] = fmaf(c, __uint_as_float(v[i]), acc[at + i]);
+      };
+      const auto half = [&](int h, float c, auto last) {
+        const int buf = 2 * turn + h;
+        tmem_ld_wait_for(d[0]);
+        tmem_ld_32x32(tmem + buf * COLS + side * 64 + 32 + lanes, d[1]);
+        add(64 * h, c, d[0]);
+        tmem_ld_wait_for(d[1]);
+        release(buf);
+        if (h == 1 && ++turn == 2) {
+          turn = 0;
           tphase ^= 1u;
         }
+        if constexpr (!last.value) begin(2 * turn + (h ^ 1));
+        add(64 * h + 32, c, d[1]);
+      };
+      begin(2 * turn);
+#pragma unroll 1
+      for (int kb = 1; kb < p.blocks_k; ++kb) {
+        const float c0 = xn * wn0, c1 = xn * wn1;
+        xn = sc.x[kb];
+        wn0 = sc.w0[kb];
+        wn1 = sc.w1[kb];
+        half(0, c0, std::false_type());
+        half(1, c1, std::false_type());
       }
+      half(0, xn * wn0, std::false_type());
+      half(1, xn * wn1, std::true_type());
+      ok = all_got(ok);
       if (!ok) break;
-      const int r_in8 = lane >> 2, piece = lane & 3;  // reading the staged rows: eight at a time, four lanes each
+      const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
+      const int rows = min(max(tl.row_end - row0, 0), 32);
+      if (t + step < total) {  // the next tile's first scales are asked for before this one is stored
+        tl = tile_at<GATED>(p, t + step);
+        sc = scales_of(tl);
+        xn = sc.x[0];
+        wn0 = sc.w0[0];
+        wn1 = sc.w1[0];
+      }
       if constexpr (GATED) {
         constexpr int OUT = COLS / 2;
-        const int c0 = tl.n0 + side * OUT;
+        const int c0 = n0 + side * OUT;
         float amax = 0.f;
 #pragma unroll
         for (int i = 0; i < OUT; ++i) {
@@ -303,18 +366,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         // The two warps of a row exchange theirs through the second halves of their staging, by turns of the tiles (a warp that
         // writes for a tile has seen all of them arrive for the one before, and so read what is overwritten).
-        const uint32_t there = 2048 + (turn & 1) * 128 + lane * 4;
+        const uint32_t there = 2048 + (tiles_done & 1) * 128 + lane * 4;
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + there), "f"(amax) : "memory");
         mbar_arrive(amax_bar);
-        ok = all_got(mbar_wait(amax_bar, turn & 1, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
+        ok = all_got(mbar_wait(amax_bar, tiles_done & 1, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
         if (!ok) break;
         float other;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((warp - 2) ^ 4) * 4096 + there) : "memory");
-        const float sc = f8::scale_of(f8::max_nan(amax, other));
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((warp - 4) ^ 4) * 4096 + there) : "memory");
+        const float s = f8::scale_of(f8::max_nan(amax, other));
         // times the reciprocal: the products carry errors of their own that are larger than its
-        const float inv = 1.f / sc;
-        const int out_blocks = (half_n + 127) / 128;
-        if (side == 0 && row < tl.row_end) p.s[static_cast<long long>(row) * out_blocks + tl.n0 / 128] = sc;
+        const float inv = 1.f / s;
+        if (side == 0 && lane < rows) p.s[static_cast<long long>(row0 + lane) * ((half_n + 127) / 128) + n0 / 128] = s;
 #pragma unroll
         for (int j = 0; j < OUT / 16; ++j) {
           uint32_t v[4];
@@ -327,61 +389,91 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + r_in8, to = tl.row0 + quad * 32 + r;
+        for (int i = 0; i < 4; ++i) {  // eight rows at a time, four lanes each
+          const int r = 8 * i + (lane >> 2), piece = lane & 3;
           uint4 v;
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                        : "r"(mine + r * 64 + ((piece ^ ((r >> 1) & 3)) * 16))
                        : "memory");
-          if (to < tl.row_end && c0 + piece * 16 < half_n) *reinterpret_cast<uint4*>(p.q + static_cast<long long>(to) * half_n + c0 + piece * 16) = v;
+          if (r < rows && c0 + piece * 16 < half_n) *reinterpret_cast<uint4*>(p.q + static_cast<long long>(row0 + r) * half_n + c0 + piece * 16) = v;
         }
         __syncwarp();
       } else {
 #pragma unroll
-        for (int j = 0; j < COLS / 32; ++j) {
-          const int c0 = tl.n0 + side * COLS + j * 32;
-          if (c0 < p.N) {
+        for (int j = 0; j < COLS / 64; ++j) {  // 64 columns at a time: rows of 128 bytes, 16-byte pieces in places that differ by row
+          const int c0 = n0 + j * 128 + side * 64;
+          if (c0 >= p.N) break;
+          if (p.residual) {  // joins the sums before they are rounded: read in whole rows, too
+            if (p.vec_r && c0 + 64 <= p.N) {
+              uint4 v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128 + ((i ^ (lane & 7)) * 16)), "f"(acc[32 * j + 4 * i]),
-                           "f"(acc[32 * j + 4 * i + 1]), "f"(acc[32 * j + 4 * i + 2]), "f"(acc[32 * j + 4 * i + 3])
-                           : "memory");
-            __syncwarp();
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                v[i] = r < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + r) * p.ldr + c0 + (lane & 7) * 8) : make_uint4(0, 0, 0, 0);
+              }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * i + r_in8, to = tl.row0 + quad * 32 + r, c = c0 + piece * 8;
-              float f[8];
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(f[4 * h]), "=f"(f[4 * h + 1]), "=f"(f[4 * h + 2]), "=f"(f[4 * h + 3])
-                             : "r"(mine + r * 128 + (((2 * piece + h) ^ (r & 7)) * 16))
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + r * 128 + (((lane & 7) ^ (r & 7)) * 16)), "r"(v[i].x), "r"(v[i].y),
+                             "r"(v[i].z), "r"(v[i].w)
                              : "memory");
-              if (to < tl.row_end && c < p.N) {
-                __nv_bfloat16* dst = p.y + static_cast<long long>(to) * p.ldy + c;
-                const __nv_bfloat16* res = p.residual ? p.residual + static_cast<long long>(to) * p.ldr + c : nullptr;
-                if (p.vec_ok && c + 8 <= p.N) {
-                  if (res) {
-                    const uint4 raw = *reinterpret_cast<const uint4*>(res);
-                    const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                      const float2 a = __bfloat1622float2(b[k]);
-                      f[2 * k] += a.x;
-                      f[2 * k + 1] += a.y;
-                    }
-                  }
-                  *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-                } else {
-#pragma unroll
-                  for (int k = 0; k < 8; ++k)
-                    if (c + k < p.N) dst[k] = __float2bfloat16(f[k] + (res ? __bfloat162float(res[k]) : 0.f));
-                }
+              }
+            } else {
+#pragma unroll 4
+              for (int i = 0; i < 64; ++i) {
+                const int r = i >> 1, c = (i & 1) * 32 + lane;
+                unsigned short v = 0;
+                if (r < rows && c0 + c < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c0 + c];
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(mine + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2), "h"(v) : "memory");
               }
             }
             __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint4 v;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                           : "r"(mine + lane * 128 + ((i ^ (lane & 7)) * 16))
+                           : "memory");
+              const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = __bfloat1622float2(b[k]);
+                acc[64 * j + 8 * i + 2 * k] += f.x;
+                acc[64 * j + 8 * i + 2 * k + 1] += f.y;
+              }
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float* f = acc + 64 * j + 8 * i;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128 + ((i ^ (lane & 7)) * 16)), "r"(pack_bf16(f[0], f[1])),
+                         "r"(pack_bf16(f[2], f[3])), "r"(pack_bf16(f[4], f[5])), "r"(pack_bf16(f[6], f[7]))
+                         : "memory");
+          }
+          __syncwarp();
+          if (p.vec_y && c0 + 64 <= p.N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              uint4 v;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                           : "r"(mine + r * 128 + (((lane & 7) ^ (r & 7)) * 16))
+                           : "memory");
+              if (r < rows) *reinterpret_cast<uint4*>(p.y + static_cast<long long>(row0 + r) * p.ldy + c0 + (lane & 7) * 8) = v;
+            }
+          } else {
+#pragma unroll 4
+            for (int i = 0; i < 64; ++i) {
+              const int r = i >> 1, c = (i & 1) * 32 + lane;
+              unsigned short v;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(mine + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2) : "memory");
+              if (r < rows && c0 + c < p.N) reinterpret_cast<unsigned short*>(p.y)[static_cast<long long>(row0 + r) * p.ldy + c0 + c] = v;
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -389,10 +481,66 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other's products, copies or arrivals may reach it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
+}
+
+// Row tiles of up to 256 rows from those of up to 128: a tile of whole 128 rows takes its successor along if that is the same expert's
+// and begins where it ends. One block goes through the list, 1024 at a time: where a run of such tiles began tells whether a tile is
+// the first of two.
+__global__ void __launch_bounds__(1024)
+pair_tiles_kernel(const int* __restrict__ tile_group, const int* __restrict__ num_tiles, int max_tiles, int groups, int M, int4* __restrict__ out,
+                  int* __restrict__ count) {
+  __shared__ int run_s[32], taken_s[32];
+  const int n = min(max(*num_tiles, 0), max_tiles), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto entry = [&](int i) {
+    int4 e = reinterpret_cast<const int4*>(tile_group)[i];
+    e.x = min(max(e.x, 0), groups - 1);
+    e.y = min(max(e.y, 0), M);
+    e.z = min(min(max(e.z, 0), BM), M - e.y);
+    return e;
+  };
+  const auto follows = [](const int4& a, const int4& b) { return a.x == b.x && a.z == BM && b.y == a.y + BM; };
+  int run_before = 0, taken_before = 0;
+  for (int i0 = 0; i0 < n; i0 += 1024) {
+    const int i = i0 + threadIdx.x;
+    int4 e = make_int4(0, 0, 0, 0), next = e;
+    bool starts = false, more = false;
+    if (i < n) {
+      e = entry(i);
+      starts = i == 0 || !follows(entry(i - 1), e);
+      if (i + 1 < n) {
+        next = entry(i + 1);
+        more = follows(e, next);
+      }
+    }
+    int run = starts ? i : 0;  // the latest start so far
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run = max(run, v);
+    }
+    if (lane == 31) run_s[warp] = run;
+    __syncthreads();
+    run = max(run, run_before);
+    for (int w = 0; w < warp; ++w) run = max(run, run_s[w]);
+    const bool take = i < n && ((i - run) & 1) == 0;
+    const unsigned ballot = __ballot_sync(0xffffffffu, take);
+    if (lane == 0) taken_s[warp] = __popc(ballot);
+    __syncthreads();
+    int at = taken_before + __popc(ballot & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) at += taken_s[w];
+    if (take) out[at] = make_int4(e.x, e.y, e.z + (more ? next.z : 0), 0);
+    for (int w = 0; w < 32; ++w) {
+      run_before = max(run_before, run_s[w]);
+      taken_before += taken_s[w];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = taken_before;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -464,40 +612,59 @@ Args args_of(const Fp8Gemm& g) {
   a.ws = g.ws;
   a.groups = g.groups;
   a.max_tiles = g.max_tiles;
-  a.tile_group = g.tile_group;
-  a.num_tiles = g.num_tiles;
   a.y = static_cast<__nv_bfloat16*>(g.y);
   a.ldy = g.ldy;
   a.residual = static_cast<const __nv_bfloat16*>(g.residual);
   a.ldr = g.ldr;
-  a.vec_ok = (g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0 &&
-              (!g.residual || (g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0))) ? 1 : 0;
+  a.vec_y = g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+  a.vec_r = g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0;
   a.q = g.q;
   a.s = g.s;
   a.status = g.status;
   return a;
 }
 
-template <int BN, bool GATED>
+template <bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
-  constexpr int STAGES = BN == 256 ? 4 : 6;
-  constexpr int SMEM = STAGES * (BM + BN) * BK + STAGING + 1024;
+  constexpr int SMEM = STAGES * STAGE + STAGING + 1024;
   CUtensorMap mx, mw;
   if (make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
-  if (make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, 128)) return -1;
+  if (make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, 64)) return -1;
   int sms = 0;
   const int dev = device_and_sms(&sms);
   static std::atomic<unsigned long long> asked{0};
-  auto kernel = fp8_gemm_kernel<BN, GATED, STAGES>;
+  auto kernel = fp8_gemm_kernel<GATED>;
   if (allow_smem(kernel, SMEM, asked, dev)) return -1;
-  const Args a = args_of(g);
-  const long long m_tiles = g.tile_group ? g.max_tiles : (g.M + BM - 1) / BM;
+  Args a = args_of(g);
+  if (g.tile_group) {
+    a.tiles = reinterpret_cast<const int4*>(g.workspace);
+    a.num_tiles = static_cast<const int*>(g.workspace) + 4ll * g.max_tiles;
+    pair_tiles_kernel<<<1, 1024, 0, stream>>>(g.tile_group, g.num_tiles, g.max_tiles, g.groups, g.M, static_cast<int4*>(g.workspace),
+                                              static_cast<int*>(g.workspace) + 4ll * g.max_tiles);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(std::string("pair_tiles launch failed: ") + cudaGetErrorString(e));
+  }
+  const long long m_tiles = g.tile_group ? g.max_tiles : (g.M + 2 * BM - 1) / (2 * BM);
   const int cols = GATED ? BN / 2 : BN;
   const long long tiles = m_tiles * ((g.N / a.halves + cols - 1) / cols);
-  if (tiles > 0x7fffffffll) return fail("too many tiles");
-  kernel<<<static_cast<int>(tiles < sms ? tiles : sms), THREADS, SMEM, stream>>>(mx, mw, a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));
+  if (tiles > 0x3fffffffll) return fail("too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < sms / 2 ? tiles : sms / 2)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // (reported here)
+    return fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));
+  }
   return 0;
 }
 
@@ -505,12 +672,12 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
 
 const char* fp8_last_error() { return g_err.c_str(); }
 
+long long fp8_gemm_workspace(const Fp8Gemm& g) { return g.tile_group ? 16ll * g.max_tiles + 16 : 0; }
+
 int fp8_gemm_launch(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.M <= 0 || g.N <= 0) return 0;
   if (g.tile_group && g.max_tiles <= 0) return 0;
-  if (g.q) return launch<256, true>(g, stream);
-  const long long m_tiles = g.tile_group ? g.max_tiles : (g.M + BM - 1) / BM;
-  return m_tiles * ((g.N + 255) / 256) >= 148 ? launch<256, false>(g, stream) : launch<128, false>(g, stream);
+  return g.q ? launch<true>(g, stream) : launch<false>(g, stream);
 }
 
 }  // namespace mb

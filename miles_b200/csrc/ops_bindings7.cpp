@@ -169,6 +169,16 @@ mb::Fp8Gemm product(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor
   return p;
 }
 
+// Launches with a workspace of the allocator's, which a captured graph keeps to itself.
+void launch(mb::Fp8Gemm& p, const at::Tensor& like, const char* name) {
+  at::Tensor ws;
+  if (const long long bytes = mb::fp8_gemm_workspace(p)) {
+    ws = at::empty({bytes}, like.options().dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+  }
+  TORCH_CHECK(mb::fp8_gemm_launch(p, cur_stream()) == 0, name, ": ", mb::fp8_last_error());
+}
+
 at::Tensor fp8_linear(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor& wq, const at::Tensor& ws, int64_t halves, const OptTensor& residual,
                       const OptTensor& tile_group, const OptTensor& num_tiles, const OptTensor& out, const OptTensor& status) {
   mb::Fp8Gemm p = product(xq, xs, wq, ws, false, halves, tile_group, num_tiles, status);
@@ -186,7 +196,7 @@ at::Tensor fp8_linear(const at::Tensor& xq, const at::Tensor& xs, const at::Tens
   at::Tensor y = out.has_value() ? *out : at::empty({p.M, p.N}, xs.options().dtype(at::kBFloat16));
   p.y = y.data_ptr();
   p.ldy = pitch(y);
-  TORCH_CHECK(mb::fp8_gemm_launch(p, cur_stream()) == 0, "fp8_linear: ", mb::fp8_last_error());
+  launch(p, xs, "fp8_linear");
   return y;
 }
 
@@ -197,7 +207,7 @@ std::tuple<at::Tensor, at::Tensor> fp8_gated_linear(const at::Tensor& xq, const 
   auto [q, s] = new_rows(p.M, p.N / 2, xq);
   p.q = static_cast<uint8_t*>(q.data_ptr());
   p.s = s.data_ptr<float>();
-  TORCH_CHECK(mb::fp8_gemm_launch(p, cur_stream()) == 0, "fp8_gated_linear: ", mb::fp8_last_error());
+  launch(p, xs, "fp8_gated_linear");
   return {q, s};
 }
 
