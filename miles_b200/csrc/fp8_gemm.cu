@@ -22,14 +22,10 @@
 #include <cuda.h>
 #include <string.h>
 
-#include <atomic>
 #include <mutex>
-#include <string>
 #include <type_traits>
 
-#include "fp8_block.h"
-#include "fp8_math.cuh"
-#include "ptx.cuh"
+#include "fp8_tile.cuh"
 
 namespace mb {
 namespace {
@@ -60,12 +56,6 @@ struct Args {
   int* status;
 };
 
-// An arrival that publishes no memory: a TMEM buffer is handed back, whose loads are complete and ordered by the fence before. (With
-// .release.cluster the second CTA's arrival waits 1200 to 1900 clocks for the thread's other accesses.)
-__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 struct Tile {
   int row0, row_end, n0, group;  // rows of x; first column of y (or of silu(gate) * up)
 };
@@ -81,24 +71,6 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Instruction descriptor of kind::f8f6f4: fp32 accumulators (bit 4), E4M3 operands (0 at bits 7 and 10), both K-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
-  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
-}
-
-// The wait of a load from TMEM names its registers, so that nothing that reads them moves ahead of it while the next load is under way.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
-                 "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
-               :
-               : "memory");
-  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
-}
-// Whether every thread of the warp came out of its wait: the loads from TMEM behind it are the whole warp's.
-__device__ __forceinline__ bool all_got(bool got) { return __all_sync(0xffffffffu, got); }
-
 template <bool GATED>
 __device__ __forceinline__ int column_tiles(const Args& p) {
   constexpr int W = GATED ? BN / 2 : BN;
@@ -231,7 +203,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       // descriptors, so its waits would leave the tensor core idle between blocks. (elect.sync tells the compiler that one thread
       // issues: under `lane == 0` a block takes 1040 clocks instead of 512.)
       if (rank == 0 && elect_one()) {
-        constexpr uint32_t idesc = idesc_e4m3(2 * BM, COLS);
+        constexpr uint32_t idesc = f8::idesc_e4m3(2 * BM, COLS);
         const int turn = warp - 1;  // buffers 0 and 1, or 2 and 3; every second stage
         const long long blocks = first_tile < total ? static_cast<long long>((total - 1 - first_tile) / step + 1) * p.blocks_k : 0;
         int stage = turn;
@@ -283,7 +255,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const uint32_t tempty0 = map_to_rank(tempty_bar(0), 0);
     const auto release = [&](int buf) {
       tc_fence_before();
-      if (lane == 0) arrive_relaxed(tempty0 + 8u * buf);
+      if (lane == 0) f8::arrive_relaxed(tempty0 + 8u * buf);
     };
     int turn = 0, tiles_done = 0;
     uint32_t tphase = 0;
@@ -317,10 +289,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       };
       const auto half = [&](int h, float c, auto last) {
         const int buf = 2 * turn + h;
-        tmem_ld_wait_for(d[0]);
+        f8::tmem_ld_wait_for(d[0]);
         tmem_ld_32x32(tmem + buf * COLS + side * 64 + 32 + lanes, d[1]);
         add(64 * h, c, d[0]);
-        tmem_ld_wait_for(d[1]);
+        f8::tmem_ld_wait_for(d[1]);
         release(buf);
         if (h == 1 && ++turn == 2) {
           turn = 0;
@@ -341,7 +313,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
       half(0, xn * wn0, std::false_type());
       half(1, xn * wn1, std::true_type());
-      ok = all_got(ok);
+      ok = f8::all_got(ok);
       if (!ok) break;
       const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
       const int rows = min(max(tl.row_end - row0, 0), 32);
@@ -369,7 +341,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         const uint32_t there = 2048 + (tiles_done & 1) * 128 + lane * 4;
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + there), "f"(amax) : "memory");
         mbar_arrive(amax_bar);
-        ok = all_got(mbar_wait(amax_bar, tiles_done & 1, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
+        ok = f8::all_got(mbar_wait(amax_bar, tiles_done & 1, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
         if (!ok) break;
         float other;
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((warp - 4) ^ 4) * 4096 + there) : "memory");
@@ -549,44 +521,33 @@ EncodeTiledFn g_encode = nullptr;
 std::once_flag g_encode_once;
 thread_local std::string g_err;
 
-int fail(const std::string& m) {
+}  // namespace
+
+int fp8_fail(const std::string& m) {
   g_err = m;
   return -1;
 }
 
 // 8-bit matrix [rows, cols] with boxes of 128 columns, 128-byte swizzle; what lies outside reads as zero
-int make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long pitch, int box_rows) {
+int fp8_make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long pitch, int box_rows) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
       g_encode = reinterpret_cast<EncodeTiledFn>(fn);
   });
-  if (!g_encode) return fail("cuTensorMapEncodeTiled is not available");
+  if (!g_encode) return fp8_fail("cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1u, 1u};
   const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
+  if (r != CUDA_SUCCESS) return fp8_fail("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
   return 0;
 }
 
-// Shared memory beyond the default, asked for once per kernel and device.
-template <typename K>
-int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& asked, int dev) {
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (asked.load(std::memory_order_acquire) & bit) return 0;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    cudaGetLastError();  // (reported here)
-    return fail("cudaFuncSetAttribute(MaxDynamicSharedMemorySize) failed");
-  }
-  asked.fetch_or(bit, std::memory_order_acq_rel);
-  return 0;
-}
-
-int device_and_sms(int* sms) {
+int fp8_device(int* sms) {
   static std::atomic<int> known[64];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -598,6 +559,8 @@ int device_and_sms(int* sms) {
   *sms = n;
   return dev;
 }
+
+namespace {
 
 Args args_of(const Fp8Gemm& g) {
   Args a;
@@ -628,13 +591,13 @@ template <bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
   constexpr int SMEM = STAGES * STAGE + STAGING + 1024;
   CUtensorMap mx, mw;
-  if (make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
-  if (make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, 64)) return -1;
+  if (fp8_make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
+  if (fp8_make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, 64)) return -1;
   int sms = 0;
-  const int dev = device_and_sms(&sms);
+  const int dev = fp8_device(&sms);
   static std::atomic<unsigned long long> asked{0};
   auto kernel = fp8_gemm_kernel<GATED>;
-  if (allow_smem(kernel, SMEM, asked, dev)) return -1;
+  if (fp8_allow_smem(kernel, SMEM, asked, dev)) return -1;
   Args a = args_of(g);
   if (g.tile_group) {
     a.tiles = reinterpret_cast<const int4*>(g.workspace);
@@ -642,12 +605,12 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
     pair_tiles_kernel<<<1, 1024, 0, stream>>>(g.tile_group, g.num_tiles, g.max_tiles, g.groups, g.M, static_cast<int4*>(g.workspace),
                                               static_cast<int*>(g.workspace) + 4ll * g.max_tiles);
     const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(std::string("pair_tiles launch failed: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return fp8_fail(std::string("pair_tiles launch failed: ") + cudaGetErrorString(e));
   }
   const long long m_tiles = g.tile_group ? g.max_tiles : (g.M + 2 * BM - 1) / (2 * BM);
   const int cols = GATED ? BN / 2 : BN;
   const long long tiles = m_tiles * ((g.N / a.halves + cols - 1) / cols);
-  if (tiles > 0x3fffffffll) return fail("too many tiles");
+  if (tiles > 0x3fffffffll) return fp8_fail("too many tiles");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < sms / 2 ? tiles : sms / 2)));
   cfg.blockDim = dim3(THREADS);
@@ -663,7 +626,7 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
   if (e != cudaSuccess) {
     cudaGetLastError();  // (reported here)
-    return fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));
+    return fp8_fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));
   }
   return 0;
 }
@@ -672,11 +635,12 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
 
 const char* fp8_last_error() { return g_err.c_str(); }
 
-long long fp8_gemm_workspace(const Fp8Gemm& g) { return g.tile_group ? 16ll * g.max_tiles + 16 : 0; }
+long long fp8_gemm_workspace(const Fp8Gemm& g) { return g.tile_group && !fp8_is_skinny(g) ? 16ll * g.max_tiles + 16 : 0; }
 
 int fp8_gemm_launch(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.M <= 0 || g.N <= 0) return 0;
   if (g.tile_group && g.max_tiles <= 0) return 0;
+  if (fp8_is_skinny(g)) return fp8_skinny_launch(g, stream);
   return g.q ? launch<true>(g, stream) : launch<false>(g, stream);
 }
 
