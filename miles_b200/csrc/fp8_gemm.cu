@@ -8,14 +8,15 @@
 // weight's tile takes 128 gate rows and their 128 up rows, so that silu(gate) * up leaves as a whole block of 128 columns of 8-bit rows,
 // scaled by their largest value, without passing through memory in between.
 //
-// A pair of CTAs (`cta_group::2`) computes 256 rows x 256 columns, each CTA its 128 rows, as two products of 128 columns a block. Four of
-// those fit TMEM. That many are needed: about 630 clocks pass from the end of a product to the start of the one that may overwrite it even
-// if nobody reads it, and a reader's loads and multiply-adds take 250 more, so that two buffers of 256 columns (one CTA) leave the tensor core
-// idle for a third of the time, while four of 128 take 4 x 256 clocks to come round. One CTA alone cannot use four: its products of 128
-// columns take 417 clocks a block instead of 256.
+// A pair of CTAs (`cta_group::2`) computes 256 rows x 256 columns, each CTA its 128 rows. Per block of 128 the tensor core needs 512 clocks, and
+// what stands in its way is shared memory: 32 KB of operands arrive and 32 KB are read, 128 bytes a clock, so little else may
+// pass there. The scales of the rows, which 128 threads would fetch from 128 lines, are therefore fetched eight blocks at a time by
+// two warps that leave the products of both scales as the readers want them (32-fold fewer accesses; a block 1130 -> 850 clocks), and the
+// operands of one row tile are multiplied by one instruction over all 256 columns (two of 128 read them twice).
 //
-//   warp 0      : TMA producer (128-byte swizzle)          warps 1, 2 : tcgen05.mma issuers (1 allocates TMEM)          (3: none)
-//   warps 4..11 : sums in registers, a row and 64 columns of each half a thread, then rows of 128 bytes through shared memory
+//   warp 0      : TMA producer (128-byte swizzle)          warp 1 : TMEM allocator, tcgen05.mma issuer
+//   warps 2, 3  : scales of the rows times the weights', eight blocks ahead
+//   warps 4..19 : sums in registers, a row and 64 columns a thread, then rows of 64 bytes through shared memory
 //
 // Reference counterpart: the block-wise FP8 GEMMs of the serving engines that load its FP8 checkpoints (weight_block_size [128, 128]:
 // miles/backends/megatron_utils/megatron_to_hf/processors/quantizer_fp8.py, miles/utils/fp8_kernel.py:24-79).
@@ -31,12 +32,15 @@ namespace mb {
 namespace {
 
 constexpr int BM = 128, BN = 256, BK = 128;  // rows of a CTA, columns of its pair's tile (W rows), columns of a block
-constexpr int COLS = 128;                    // of a tile's half: a thread's
-constexpr int STAGES = 6, BUFS = 4;          // (an even number of stages: each issuer has its own)
-constexpr int X_BYTES = BM * BK, W_HALF_BYTES = 64 * BK;  // of a stage: this CTA's rows of x; its 64 W rows of each half
-constexpr int STAGE = X_BYTES + 2 * W_HALF_BYTES;
-constexpr int THREADS = 384;                 // three warpgroups: the second and third sum up, with registers that the first gives back
-constexpr int STAGING = 8 * 4096;
+constexpr int COLS = 64;                     // of a thread
+constexpr int STAGES = 5, BUFS = 2;
+constexpr int X_BYTES = BM * BK, W_BYTES = BN / 2 * BK;  // of a stage: this CTA's rows of x, and of W
+constexpr int STAGE = X_BYTES + W_BYTES;
+constexpr int EPI_WARPS = 16;
+constexpr int THREADS = 128 + 32 * EPI_WARPS;  // the first warpgroup gives registers to the others, which sum up
+constexpr int STAGING = EPI_WARPS * 2048;
+constexpr int AHEAD = 8, SLOTS = 2;          // blocks of scales in a slot
+constexpr int SLOT_BYTES = 2 * AHEAD * BM * 4;
 
 struct Args {
   int M, N, K;
@@ -50,7 +54,7 @@ struct Args {
   long long ldy;
   const __nv_bfloat16* residual;
   long long ldr;
-  int vec_y, vec_r;                // 16-byte accesses fit
+  int vec_y, vec_r, vec_s;         // 16-byte accesses fit
   uint8_t* q;
   float* s;
   int* status;
@@ -71,6 +75,15 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void st_shared(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 template <bool GATED>
 __device__ __forceinline__ int column_tiles(const Args& p) {
   constexpr int W = GATED ? BN / 2 : BN;
@@ -107,18 +120,14 @@ __device__ __forceinline__ Tile tile_at(const Args& p, int t) {
   return r;
 }
 
-// What a thread multiplies its sums' blocks with: the scales of its row, and of the weights' block(s) that its columns are in.
-struct Scales {
-  const float *x, *w0, *w1;
-};
-
 template <bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = base + STAGES * STAGE;
-  __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFS + 1];
+  const uint32_t scales = staging + STAGING;
+  __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFS + 2 * SLOTS + 1];
   __shared__ uint32_t tmem_slot_s;
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
@@ -127,7 +136,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
   auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + BUFS + b); };    // of the CTA of rank 0: both CTAs have read the buffer
-  const uint32_t amax_bar = bar0 + 8u * (2 * STAGES + 2 * BUFS);
+  auto sfull_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + 2 * BUFS + s); };
+  auto sempty_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + 2 * BUFS + SLOTS + s); };
+  const uint32_t amax_bar = bar0 + 8u * (2 * STAGES + 2 * BUFS + 2 * SLOTS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int first_tile = blockIdx.x / 2, step = gridDim.x / 2;
@@ -140,9 +151,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
     for (int b = 0; b < BUFS; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 16);  // eight warps of each CTA
+      mbar_init(tempty_bar(b), 2 * EPI_WARPS);
     }
-    mbar_init(amax_bar, 256);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(sfull_bar(s), 2);
+      mbar_init(sempty_bar(s), EPI_WARPS);
+    }
+    mbar_init(amax_bar, 32 * EPI_WARPS);
     fence_barrier_init();
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
@@ -156,9 +171,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   const int total = tiles_of<GATED>(p);
   const int half_n = p.N / p.halves;
 
-  // 4 x 32 x 56 + 8 x 32 x 224 registers are the 384 x 168 of the launch
+  // 4 x 32 x 32 + 16 x 32 x 112 registers are the 640 x 96 of the launch
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0) {
       if (elect_one()) {
         int stage = 0;
@@ -166,8 +181,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         bool ok = true;
         for (int t = first_tile; ok && t < total; t += step) {
           const Tile tl = tile_at<GATED>(p, t);
-          const int w0 = tl.group * p.N + tl.n0 + rank * 64;  // this CTA's rows of W: 64 of each half of the tile
-          const int w1 = w0 + (GATED ? half_n : 128);
+          const int w0 = tl.group * p.N + tl.n0 + rank * (GATED ? 64 : 128);  // this CTA's rows of W
           for (int kb = 0; kb < p.blocks_k; ++kb) {
             if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, ERR_WAIT_EMPTY)) {
               ok = false;
@@ -177,7 +191,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             const uint32_t full = map_to_rank(full_bar(stage), 0), dst = base + stage * STAGE;
             tma_load_2d_pair(dst, &map_x, full, kb * BK, tl.row0 + rank * BM);
             tma_load_2d_pair(dst + X_BYTES, &map_w, full, kb * BK, w0);
-            tma_load_2d_pair(dst + X_BYTES + W_HALF_BYTES, &map_w, full, kb * BK, w1);
+            if (GATED) tma_load_2d_pair(dst + X_BYTES + W_BYTES / 2, &map_w, full, kb * BK, w0 + half_n);  // the up rows of its gate rows
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -198,57 +212,97 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
       __syncwarp();
-    } else if (warp <= 2) {
-      // Two issuers, by turns of the blocks. One is not enough: it cannot prepare a block while the products it has issued still read their
-      // descriptors, so its waits would leave the tensor core idle between blocks. (elect.sync tells the compiler that one thread
-      // issues: under `lane == 0` a block takes 1040 clocks instead of 512.)
+    } else if (warp == 1) {
+      // (elect.sync tells the compiler that one thread issues: under `lane == 0` a block takes 1040 clocks instead of 512)
       if (rank == 0 && elect_one()) {
-        constexpr uint32_t idesc = f8::idesc_e4m3(2 * BM, COLS);
-        const int turn = warp - 1;  // buffers 0 and 1, or 2 and 3; every second stage
-        const long long blocks = first_tile < total ? static_cast<long long>((total - 1 - first_tile) / step + 1) * p.blocks_k : 0;
-        int stage = turn;
+        constexpr uint32_t idesc = f8::idesc_e4m3(2 * BM, BN);
+        int stage = 0, buf = 0;
         uint32_t phase = 0, tphase = 0;
         bool ok = true;
-        for (long long b = turn; ok && b < blocks; b += 2) {
-          ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, ERR_WAIT_FULL);
-          const uint32_t x = base + stage * STAGE;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ok = ok && mbar_wait(tempty_bar(2 * turn + h), tphase ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
+        for (int t = first_tile; ok && t < total; t += step) {
+          for (int kb = 0; ok && kb < p.blocks_k; ++kb) {
+            ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, ERR_WAIT_FULL) &&
+                 mbar_wait(tempty_bar(buf), tphase ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t w = x + X_BYTES + h * W_HALF_BYTES;
+            const uint32_t x = base + stage * STAGE, w = x + X_BYTES;
 #pragma unroll
             for (int k = 0; k < BK / 32; ++k)
-              umma_f8_pair(tmem + (2 * turn + h) * COLS, make_smem_desc(x + k * 32, 16, 1024), make_smem_desc(w + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
-            umma_commit_pair(tfull_bar(2 * turn + h));
-          }
-          if (!ok) break;
-          umma_commit_pair(empty_bar(stage));
-          tphase ^= 1u;
-          stage += 2;
-          if (stage >= STAGES) {
-            stage -= STAGES;
-            phase ^= 1u;
+              umma_f8_pair(tmem + buf * BN, make_smem_desc(x + k * 32, 16, 1024), make_smem_desc(w + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
+            umma_commit_pair(tfull_bar(buf));
+            umma_commit_pair(empty_bar(stage));
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            if (++buf == BUFS) {
+              buf = 0;
+              tphase ^= 1u;
+            }
           }
         }
       }
       __syncwarp();
+    } else {
+      // [slot][half of the columns, or gate and up][block][row]: this warp's 64 rows
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first_tile; ok && t < total; t += step) {
+        const Tile tl = tile_at<GATED>(p, t);
+        const int nb = tl.n0 / 128, row = tl.row0 + rank * BM + (warp - 2) * 64 + lane;
+        const float* x0 = p.xs + static_cast<long long>(min(row, p.M - 1)) * p.blocks_k;
+        const float* x1 = p.xs + static_cast<long long>(min(row + 32, p.M - 1)) * p.blocks_k;
+        const float* ws0 = p.ws + (static_cast<long long>(tl.group) * p.blocks_n + nb) * p.blocks_k;
+        const float* ws1 = ws0 + static_cast<long long>(GATED ? p.blocks_n / 2 : nb + 1 < p.blocks_n ? 1 : 0) * p.blocks_k;
+        for (int kb = 0; ok && kb < p.blocks_k; kb += AHEAD) {
+          ok = f8::all_got(mbar_wait(sempty_bar(slot), phase ^ 1u, abort_flag, p.status, ERR_WAIT_EMPTY));
+          if (!ok) break;
+          const int n = min(AHEAD, p.blocks_k - kb);
+          // lanes 0..7 the first weights' scales of the blocks, 8..15 the second's
+          const float w = lane < 2 * AHEAD && (lane & (AHEAD - 1)) < n ? (lane < AHEAD ? ws0 : ws1)[kb + (lane & (AHEAD - 1))] : 0.f;
+          const uint32_t to = scales + slot * SLOT_BYTES + ((warp - 2) * 64 + lane) * 4;
+#pragma unroll
+          for (int i = 0; i < AHEAD; i += 4) {
+            float a[4], b[4];
+            if (p.vec_s) {
+              const float4 u = i < n ? *reinterpret_cast<const float4*>(x0 + kb + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+              const float4 v = i < n ? *reinterpret_cast<const float4*>(x1 + kb + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+              a[0] = u.x, a[1] = u.y, a[2] = u.z, a[3] = u.w, b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                a[k] = i + k < n ? x0[kb + i + k] : 0.f;
+                b[k] = i + k < n ? x1[kb + i + k] : 0.f;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float w0 = __shfl_sync(0xffffffffu, w, i + k), w1 = __shfl_sync(0xffffffffu, w, AHEAD + i + k);
+              const uint32_t at = to + (i + k) * (BM * 4);
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(a[k] * w0) : "memory");
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 128), "f"(b[k] * w0) : "memory");
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + SLOT_BYTES / 2), "f"(a[k] * w1) : "memory");
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + SLOT_BYTES / 2 + 128), "f"(b[k] * w1) : "memory");
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfull_bar(slot));
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int quad = warp & 3, side = (warp - 4) >> 2;  // rows of the tile that this warp reaches in TMEM; its 64 columns of each half
-    const uint32_t mine = staging + (warp - 4) * 4096;
-    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const auto scales_of = [&](const Tile& tl) {
-      Scales r;
-      const int row = min(tl.row0 + rank * BM + quad * 32 + lane, p.M - 1);
-      const int nb = tl.n0 / 128;
-      r.x = p.xs + static_cast<long long>(row) * p.blocks_k;
-      r.w0 = p.ws + (static_cast<long long>(tl.group) * p.blocks_n + nb) * p.blocks_k;
-      r.w1 = r.w0 + static_cast<long long>(GATED ? p.blocks_n / 2 : nb + 1 < p.blocks_n ? 1 : 0) * p.blocks_k;
-      return r;
-    };
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    // rows of the tile that this warp reaches in TMEM; its part of the columns: 64 of y, or 32 of the gates and 32 of their up columns
+    const int quad = warp & 3, part = (warp - 4) >> 2, half = part >> 1;
+    const uint32_t mine = staging + (warp - 4) * 2048;
+    const uint32_t from0 = tmem + (GATED ? half * (BN / 2) + (part & 1) * 32 : part * COLS) + (static_cast<uint32_t>(quad * 32) << 16);
+    constexpr int THEN = GATED ? BN / 4 : 32;  // from its first 32 columns to the others
+    const uint32_t my_scales = scales + (GATED ? 0 : half * (SLOT_BYTES / 2)) + (quad * 32 + lane) * 4;
     // Between blocks as few instructions as can be: the additions alone take half of the clocks that the products leave. So a wait that
     // runs out is looked at once a tile (what is read meanwhile is thrown away, and every later wait ends at once), and a buffer is
     // handed back by one lane without a word from the others: the wait for their loads is the whole warp's.
@@ -257,192 +311,159 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       tc_fence_before();
       if (lane == 0) f8::arrive_relaxed(tempty0 + 8u * buf);
     };
-    int turn = 0, tiles_done = 0;
-    uint32_t tphase = 0;
+    int buf = 0, slot = 0, tiles_done = 0;
+    uint32_t tphase = 0, sphase = 0;
     bool ok = true;
-    float xn = 0.f, wn0 = 0.f, wn1 = 0.f;  // of the next block
-    Scales sc = {};
-    Tile tl = {};
-    if (first_tile < total) {
-      tl = tile_at<GATED>(p, first_tile);
-      sc = scales_of(tl);
-      xn = sc.x[0];
-      wn0 = sc.w0[0];
-      wn1 = sc.w1[0];
-    }
     for (int t = first_tile; t < total; t += step, ++tiles_done) {
-      float acc[COLS];  // 64 columns of each half
+      const Tile tl = tile_at<GATED>(p, t);
+      const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
+      const int rows = min(max(tl.row_end - row0, 0), 32);
+      float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-      // 32 columns are under way while 32 are added, from half to half and block to block. Both warps of a scheduler read a half
-      // together, so that it is handed back as soon as can be.
-      uint32_t d[2][32];
-      const auto begin = [&](int buf) {  // its first columns
+#pragma unroll 1
+      for (int kb = 0; kb < p.blocks_k; ++kb) {
+        const int in_slot = kb & (AHEAD - 1);
+        if (in_slot == 0) {
+          ok = mbar_wait(sfull_bar(slot), sphase, abort_flag, p.status, ERR_WAIT_FULL) && ok;
+          __syncwarp();
+        }
+        const uint32_t at = my_scales + slot * SLOT_BYTES + in_slot * (BM * 4);
+        float c0, c1;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c0) : "r"(at) : "memory");
+        if constexpr (GATED) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c1) : "r"(at + SLOT_BYTES / 2) : "memory");
+        else c1 = c0;
+        if (in_slot == AHEAD - 1 || kb + 1 == p.blocks_k) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty_bar(slot));
+          if (++slot == SLOTS) {
+            slot = 0;
+            sphase ^= 1u;
+          }
+        }
         ok = mbar_wait(tfull_bar(buf), tphase, abort_flag, p.status, ERR_WAIT_TMEM_FULL) && ok;
         __syncwarp();
         tc_fence_after();
-        tmem_ld_32x32(tmem + buf * COLS + side * 64 + lanes, d[0]);
-      };
-      const auto add = [&](int at, float c, const uint32_t(&v)[32]) {
+        uint32_t d[32];
+        tmem_ld_32x32(from0 + buf * BN, d);
+        f8::tmem_ld_wait_for(d);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[at + i] = fmaf(c, __uint_as_float(v[i]), acc[at + i]);
-      };
-      const auto half = [&](int h, float c, auto last) {
-        const int buf = 2 * turn + h;
-        f8::tmem_ld_wait_for(d[0]);
-        tmem_ld_32x32(tmem + buf * COLS + side * 64 + 32 + lanes, d[1]);
-        add(64 * h, c, d[0]);
-        f8::tmem_ld_wait_for(d[1]);
+        for (int i = 0; i < 32; ++i) acc[i] = fmaf(c0, __uint_as_float(d[i]), acc[i]);
+        tmem_ld_32x32(from0 + buf * BN + THEN, d);
+        f8::tmem_ld_wait_for(d);
         release(buf);
-        if (h == 1 && ++turn == 2) {
-          turn = 0;
+        if (++buf == BUFS) {
+          buf = 0;
           tphase ^= 1u;
         }
-        if constexpr (!last.value) begin(2 * turn + (h ^ 1));
-        add(64 * h + 32, c, d[1]);
-      };
-      begin(2 * turn);
-#pragma unroll 1
-      for (int kb = 1; kb < p.blocks_k; ++kb) {
-        const float c0 = xn * wn0, c1 = xn * wn1;
-        xn = sc.x[kb];
-        wn0 = sc.w0[kb];
-        wn1 = sc.w1[kb];
-        half(0, c0, std::false_type());
-        half(1, c1, std::false_type());
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[32 + i] = fmaf(c1, __uint_as_float(d[i]), acc[32 + i]);
       }
-      half(0, xn * wn0, std::false_type());
-      half(1, xn * wn1, std::true_type());
       ok = f8::all_got(ok);
       if (!ok) break;
-      const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
-      const int rows = min(max(tl.row_end - row0, 0), 32);
-      if (t + step < total) {  // the next tile's first scales are asked for before this one is stored
-        tl = tile_at<GATED>(p, t + step);
-        sc = scales_of(tl);
-        xn = sc.x[0];
-        wn0 = sc.w0[0];
-        wn1 = sc.w1[0];
-      }
       if constexpr (GATED) {
         constexpr int OUT = COLS / 2;
-        const int c0 = n0 + side * OUT;
+        const int c0 = n0 + part * OUT;
         float amax = 0.f;
 #pragma unroll
         for (int i = 0; i < OUT; ++i) {
           const float g = acc[i];
-          // (__expf is exact to 2 + |g| / 10 units in the last place, where the sums before it are to about 10)
-          const float a = c0 + i < half_n ? g / (1.f + __expf(-g)) * acc[OUT + i] : 0.f;
+          // (__expf and __fdividef are exact to a few units in the last place, where the sums before them are to about 10; where the divisor
+          // is above 2^126 the quotient is zero as it should be in fp32, less 1e-37)
+          const float a = c0 + i < half_n ? __fdividef(g, 1.f + __expf(-g)) * acc[OUT + i] : 0.f;
           acc[i] = a;
           amax = f8::max_nan(amax, fabsf(a));
         }
-        // The two warps of a row exchange theirs through the second halves of their staging, by turns of the tiles (a warp that
+        // The four warps of a row exchange theirs through the second halves of their staging, by turns of the tiles (a warp that
         // writes for a tile has seen all of them arrive for the one before, and so read what is overwritten).
-        const uint32_t there = 2048 + (tiles_done & 1) * 128 + lane * 4;
+        const uint32_t there = 1024 + (tiles_done & 1) * 128 + lane * 4;
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + there), "f"(amax) : "memory");
         mbar_arrive(amax_bar);
         ok = f8::all_got(mbar_wait(amax_bar, tiles_done & 1, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
         if (!ok) break;
-        float other;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((warp - 4) ^ 4) * 4096 + there) : "memory");
-        const float s = f8::scale_of(f8::max_nan(amax, other));
+#pragma unroll
+        for (int k = 1; k < 4; ++k) {
+          float other;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((part ^ k) * 4 + quad) * 2048 + there) : "memory");
+          amax = f8::max_nan(amax, other);
+        }
+        const float s = f8::scale_of(amax);
         // times the reciprocal: the products carry errors of their own that are larger than its
         const float inv = 1.f / s;
-        if (side == 0 && lane < rows) p.s[static_cast<long long>(row0 + lane) * ((half_n + 127) / 128) + n0 / 128] = s;
+        if (part == 0 && lane < rows) p.s[static_cast<long long>(row0 + lane) * ((half_n + 127) / 128) + n0 / 128] = s;
 #pragma unroll
         for (int j = 0; j < OUT / 16; ++j) {
           uint32_t v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             v[i] = f8::pack_e4m3(acc[16 * j + 4 * i] * inv, acc[16 * j + 4 * i + 1] * inv, acc[16 * j + 4 * i + 2] * inv, acc[16 * j + 4 * i + 3] * inv);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                       "r"(v[3])
-                       : "memory");
+          st_shared(mine + lane * 32 + ((j ^ ((lane >> 2) & 1)) * 16), make_uint4(v[0], v[1], v[2], v[3]));
         }
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // eight rows at a time, four lanes each
-          const int r = 8 * i + (lane >> 2), piece = lane & 3;
-          uint4 v;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                       : "r"(mine + r * 64 + ((piece ^ ((r >> 1) & 3)) * 16))
-                       : "memory");
+        for (int i = 0; i < 2; ++i) {  // sixteen rows at a time, two lanes each
+          const int r = 16 * i + (lane >> 1), piece = lane & 1;
+          const uint4 v = ld_shared(mine + r * 32 + ((piece ^ ((r >> 2) & 1)) * 16));
           if (r < rows && c0 + piece * 16 < half_n) *reinterpret_cast<uint4*>(p.q + static_cast<long long>(row0 + r) * half_n + c0 + piece * 16) = v;
         }
         __syncwarp();
       } else {
 #pragma unroll
-        for (int j = 0; j < COLS / 64; ++j) {  // 64 columns at a time: rows of 128 bytes, 16-byte pieces in places that differ by row
-          const int c0 = n0 + j * 128 + side * 64;
+        for (int j = 0; j < 2; ++j) {  // 32 columns at a time: rows of 64 bytes, 16-byte pieces in places that differ by row
+          const int c0 = n0 + part * COLS + j * 32;
           if (c0 >= p.N) break;
-          if (p.residual) {  // joins the sums before they are rounded: read in whole rows, too
-            if (p.vec_r && c0 + 64 <= p.N) {
-              uint4 v[8];
+          const auto place = [&](int r, int piece) { return mine + r * 64 + ((piece ^ ((r >> 1) & 3)) * 16); };
+          const auto element = [&](int r) { return place(r, lane >> 3) + (lane & 7) * 2; };
+          const int r8 = lane >> 2, piece = lane & 3;  // whole rows: eight at a time, four lanes each
+          if (p.residual) {                            // joins the sums before they are rounded: read in whole rows, too
+            if (p.vec_r && c0 + 32 <= p.N) {
+              uint4 v[4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                v[i] = r < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + r) * p.ldr + c0 + (lane & 7) * 8) : make_uint4(0, 0, 0, 0);
-              }
+              for (int i = 0; i < 4; ++i)
+                v[i] = 8 * i + r8 < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + 8 * i + r8) * p.ldr + c0 + piece * 8)
+                                         : make_uint4(0, 0, 0, 0);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + r * 128 + (((lane & 7) ^ (r & 7)) * 16)), "r"(v[i].x), "r"(v[i].y),
-                             "r"(v[i].z), "r"(v[i].w)
-                             : "memory");
-              }
+              for (int i = 0; i < 4; ++i) st_shared(place(8 * i + r8, piece), v[i]);
             } else {
 #pragma unroll 4
-              for (int i = 0; i < 64; ++i) {
-                const int r = i >> 1, c = (i & 1) * 32 + lane;
+              for (int r = 0; r < 32; ++r) {
                 unsigned short v = 0;
-                if (r < rows && c0 + c < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c0 + c];
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(mine + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2), "h"(v) : "memory");
+                if (r < rows && c0 + lane < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c0 + lane];
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r)), "h"(v) : "memory");
               }
             }
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint4 v;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                           : "r"(mine + lane * 128 + ((i ^ (lane & 7)) * 16))
-                           : "memory");
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = ld_shared(place(lane, i));
               const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&v);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float2 f = __bfloat1622float2(b[k]);
-                acc[64 * j + 8 * i + 2 * k] += f.x;
-                acc[64 * j + 8 * i + 2 * k + 1] += f.y;
+                acc[32 * j + 8 * i + 2 * k] += f.x;
+                acc[32 * j + 8 * i + 2 * k + 1] += f.y;
               }
             }
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float* f = acc + 64 * j + 8 * i;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128 + ((i ^ (lane & 7)) * 16)), "r"(pack_bf16(f[0], f[1])),
-                         "r"(pack_bf16(f[2], f[3])), "r"(pack_bf16(f[4], f[5])), "r"(pack_bf16(f[6], f[7]))
-                         : "memory");
+          for (int i = 0; i < 4; ++i) {
+            const float* f = acc + 32 * j + 8 * i;
+            st_shared(place(lane, i), make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
           }
           __syncwarp();
-          if (p.vec_y && c0 + 64 <= p.N) {
+          if (p.vec_y && c0 + 32 <= p.N) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3);
-              uint4 v;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                           : "r"(mine + r * 128 + (((lane & 7) ^ (r & 7)) * 16))
-                           : "memory");
-              if (r < rows) *reinterpret_cast<uint4*>(p.y + static_cast<long long>(row0 + r) * p.ldy + c0 + (lane & 7) * 8) = v;
+            for (int i = 0; i < 4; ++i) {
+              const int r = 8 * i + r8;
+              const uint4 v = ld_shared(place(r, piece));
+              if (r < rows) *reinterpret_cast<uint4*>(p.y + static_cast<long long>(row0 + r) * p.ldy + c0 + piece * 8) = v;
             }
           } else {
 #pragma unroll 4
-            for (int i = 0; i < 64; ++i) {
-              const int r = i >> 1, c = (i & 1) * 32 + lane;
+            for (int r = 0; r < 32; ++r) {
               unsigned short v;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(mine + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2) : "memory");
-              if (r < rows && c0 + c < p.N) reinterpret_cast<unsigned short*>(p.y)[static_cast<long long>(row0 + r) * p.ldy + c0 + c] = v;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(element(r)) : "memory");
+              if (r < rows && c0 + lane < p.N) reinterpret_cast<unsigned short*>(p.y)[static_cast<long long>(row0 + r) * p.ldy + c0 + lane] = v;
             }
           }
           __syncwarp();
@@ -581,6 +602,7 @@ Args args_of(const Fp8Gemm& g) {
   a.ldr = g.ldr;
   a.vec_y = g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
   a.vec_r = g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0;
+  a.vec_s = a.blocks_k % 4 == 0 && (reinterpret_cast<uintptr_t>(g.xs) & 15) == 0;
   a.q = g.q;
   a.s = g.s;
   a.status = g.status;
@@ -589,10 +611,10 @@ Args args_of(const Fp8Gemm& g) {
 
 template <bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
-  constexpr int SMEM = STAGES * STAGE + STAGING + 1024;
+  constexpr int SMEM = STAGES * STAGE + STAGING + SLOTS * SLOT_BYTES + 1024;
   CUtensorMap mx, mw;
   if (fp8_make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
-  if (fp8_make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, 64)) return -1;
+  if (fp8_make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, GATED ? 64 : 128)) return -1;
   int sms = 0;
   const int dev = fp8_device(&sms);
   static std::atomic<unsigned long long> asked{0};
