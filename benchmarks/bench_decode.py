@@ -30,6 +30,7 @@ def main() -> None:
     ap.add_argument("--ctx", type=int, default=2000)
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--hbm-gbs", type=float, default=None)
+    ap.add_argument("--quantization", default="none", choices=["none", "mxfp8", "nvfp4", "fp8_block"], help="serve from such copies of the weights (bytes and floor stay those of bf16)")
     ns = ap.parse_args()
 
     from clocks import ClockSampler
@@ -47,6 +48,8 @@ def main() -> None:
     cfg.num_layers = ns.layers
     store = ParamStore(cfg, dev, torch.bfloat16)
     model = build_model(cfg, store, "b200")
+    if ns.quantization != "none":
+        model.enable_block_scaled(ns.quantization)
     batches = [int(b) for b in ns.batches.split(",")]
     eng = Engine(model, max_running=max(batches), page_size=64, max_seq_len=ns.ctx + ns.steps * 4 + 64, use_cuda_graph=True)
     g = torch.Generator().manual_seed(0)
@@ -83,7 +86,7 @@ def main() -> None:
         layer_bytes += B * ns.ctx * 2 * cfg.num_kv_heads * D * 2
         head_bytes = cfg.vocab_size * H * 2
         floor_ms = (ns.layers * layer_bytes + head_bytes) / (hbm * 1e9) * 1e3
-        print(json.dumps({"what": "decode_step", "model": ns.model, "layers": ns.layers, "batch": B, "ctx": ns.ctx, "ms_per_step": ms,
+        print(json.dumps({"what": "decode_step", "model": ns.model, "quantization": ns.quantization, "layers": ns.layers, "batch": B, "ctx": ns.ctx, "ms_per_step": ms,
                           "us_per_layer": (ms - head_bytes / (hbm * 1e9) * 1e3) * 1e3 / ns.layers, "layer_mbytes": layer_bytes / 1e6,
                           "hbm_floor_ms": floor_ms, "frac_of_measured_hbm": floor_ms / ms,
                           "clocks": clocks}), flush=True)

@@ -27,6 +27,8 @@ struct Fp8Gemm {
   void* workspace;    // fp8_gemm_workspace bytes, 16-byte aligned
 };
 long long fp8_gemm_workspace(const Fp8Gemm& p);
+// Launches of a product by expert: one, and one to join row tiles where the rows are many.
+int fp8_grouped_launches(long long rows, int groups);
 // Launches on `stream`. Returns 0 or -1 with the reason in fp8_last_error().
 int fp8_gemm_launch(const Fp8Gemm& p, cudaStream_t stream);
 const char* fp8_last_error();

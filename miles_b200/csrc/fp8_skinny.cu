@@ -432,6 +432,15 @@ bool fp8_is_skinny(const Fp8Gemm& g) {
   return g.M <= 128 || pairs < 60;
 }
 
+int fp8_grouped_launches(long long rows, int groups) {
+  Fp8Gemm g{};
+  g.M = static_cast<int>(rows);
+  g.groups = groups;
+  static const int some = 0;
+  g.tile_group = &some;
+  return fp8_is_skinny(g) ? 1 : 2;
+}
+
 int fp8_skinny_launch(const Fp8Gemm& g, cudaStream_t stream) {
   const long long rows = g.tile_group ? g.M / (g.groups < g.M ? g.groups : g.M) : g.M;  // of a tile, or an expert's on average
   if (g.q) return rows <= 16 ? launch<16, true>(g, stream) : rows <= 32 ? launch<32, true>(g, stream) : launch<64, true>(g, stream);

@@ -200,7 +200,7 @@ def build_from_args(argv=None):
     ap.add_argument("--page-size", type=int, default=64)
     ap.add_argument("--context-length", type=int, default=9224)
     ap.add_argument("--mem-fraction-static", type=float, default=0.85)
-    ap.add_argument("--quantization", default="none", choices=["none", "mxfp8", "nvfp4"])
+    ap.add_argument("--quantization", default="none", choices=["none", "mxfp8", "nvfp4", "fp8_block"])
     ap.add_argument("--dtype", default="auto", choices=["auto", "bfloat16", "float32"],
                     help="auto: bfloat16 on a GPU, float32 on the CPU; float32 on a GPU is built for models with a layer plan")
     ap.add_argument("--max-prefill-tokens", type=int, default=16384, help="tokens of one prefill pass; planned-layer models compute longer prompts in portions")

@@ -188,9 +188,12 @@ class B200Qwen3:
 
     def enable_block_scaled(self, kind: str) -> int:
         """Serve the projections and experts from MXFP8 / NVFP4 copies of the weights (`csrc/gemm_mx.cu`) whenever
-        more than 32 rows are multiplied; the few-row decode kernels keep streaming the bf16 weights. Meant for a
+        more than 32 rows are multiplied, or from E4M3 copies with a scale for each 128 x 128 (``fp8_block``, `ops/fp8_block.py`) whenever more
+        than ``SMALL_T`` are; the few-row decode kernels keep streaming the bf16 weights. Meant for a
         model object that only the rollout engine uses. Call again (or `refresh_block_scaled`) after a weight update.
         Returns the number of tensors quantised."""
+        if kind == "fp8_block":
+            return self._enable_fp8_block()
         from ..ops.mx_gemm import quantize_operand
 
         step = 128 if kind == "mxfp8" else 256
@@ -204,6 +207,38 @@ class B200Qwen3:
             self.mx[w.data_ptr()] = quantize_operand(w2, kind)
         return len(self.mx)
 
+    def _enable_fp8_block(self) -> int:
+        from ..ops.fp8_block import quantize_weight
+
+        old = self.mx if getattr(self, "mx_kind", None) == "fp8_block" else {}
+        self.mx_kind, self.mx = "fp8_block", {}
+        for name, w in self.store.params.items():
+            halves = 2 if name.endswith(("mlp.gate_up.weight", "moe.w1")) else 1
+            # (rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a gate-up product leaves)
+            if not name.endswith(self.MX_SUFFIXES) or w.shape[-1] % 16 or w.shape[-2] % (16 * halves):
+                continue
+            q = quantize_weight(w, halves)
+            kept = old.get(w.data_ptr())
+            if kept is not None and kept.q.shape == q.q.shape:  # captured decode steps read the copies where they were
+                kept.q.view(torch.uint8).copy_(q.q.view(torch.uint8))
+                kept.scales.copy_(q.scales)
+                q = kept
+            self.mx[w.data_ptr()] = q
+        return len(self.mx)
+
+    def _fp8(self, w, rows: int):
+        """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None. us, one dense layer's products with their norms and
+        activation, bf16 / 8 bits: see DECODE."""
+        mx = getattr(self, "mx", None)
+        return mx.get(w.data_ptr()) if mx and self.mx_kind == "fp8_block" and rows > self.SMALL_T else None
+
+    def _fp8_layer(self, i: int, rows: int) -> bool:
+        """Whether layer i's activations pass from product to product in 8 bits: not where they are exchanged with other ranks or normed once more."""
+        if self.tp is not None or self.ep is not None or self.cfg.post_norms or not getattr(self, "mx", None):
+            return False
+        names = ("moe.w1", "moe.w2") if self.cfg.layer_is_moe(i) else ("mlp.gate_up.weight", "mlp.down.weight")
+        return all(self._fp8(self.store.params[f"layers.{i}.{n}"], rows) is not None for n in ("attn.qkv.weight", "attn.o.weight", *names))
+
     def use_block_scaled(self, kind: str, operands: dict) -> None:
         """Serve from block-scaled copies that something else keeps up to date (``{parameter name: MxOperand}``, e.g.
         the buffers a peer-memory weight push quantises into)."""
@@ -215,6 +250,12 @@ class B200Qwen3:
             return
         if getattr(self, "mx", None):
             self.enable_block_scaled(self.mx_kind)
+
+    def _fp8_linear(self, x, w8, residual=None):
+        from ..ops import fp8_block as F8
+
+        self.launches += 1 if isinstance(x, F8.Fp8Rows) else 2
+        return F8.linear(x, w8, residual, status=self.status)
 
     def _mx_linear(self, x, wq, tile_group=None, num_tiles=None, n: int = 0, amax=None):
         from ..ops.mx_gemm import mx_linear, quantize_operand
@@ -230,7 +271,11 @@ class B200Qwen3:
         engine (``serving``) may split the contraction of up to 128 rows over a cluster (csrc/gemm_skinny.cu)."""
         T, (N, K) = x.shape[0], w.shape
         mx = getattr(self, "mx", None)
-        if mx and T > 32 and out_dtype == torch.bfloat16 and w.data_ptr() in mx:
+        if mx and out_dtype == torch.bfloat16 and self.mx_kind == "fp8_block":
+            w8 = self._fp8(w, T)
+            if w8 is not None:
+                return self._fp8_linear(x, w8)
+        elif mx and T > 32 and out_dtype == torch.bfloat16 and w.data_ptr() in mx:
             return self._mx_linear(x.contiguous(), mx[w.data_ptr()])
         out = torch.empty(x.shape[0], w.shape[0], dtype=out_dtype, device=x.device)
         if T <= 8 and self.small_decode and N % 16 == 0 and K % 32 == 0 and N * K * 2 < (48 << 20) and x.is_contiguous():
@@ -305,7 +350,11 @@ class B200Qwen3:
         C = self.C
         I2 = w1.shape[1]
         mx = getattr(self, "mx", None)
-        if mx and not keep and scatter is None and w1.data_ptr() in mx and w2.data_ptr() in mx and plan.align == 128:
+        if mx and self.mx_kind == "fp8_block":
+            tokens = plan.ids.shape[0]
+            if not keep and scatter is None and self._fp8(w1, tokens) is not None and self._fp8(w2, tokens) is not None:
+                return None, None, self._fp8_experts(xp, plan, w1, w2)
+        elif mx and not keep and scatter is None and w1.data_ptr() in mx and w2.data_ptr() in mx and plan.align == 128:
             # rows of xp past the live tiles are never written: the per-tensor scale of NVFP4 must not look at them
             gu = self._mx_linear(xp, mx[w1.data_ptr()], plan.tile_group, plan.num_tiles, I2, getattr(plan, "amax_in", None))
             act = C.swiglu_fwd(gu)
@@ -330,7 +379,20 @@ class B200Qwen3:
         self.launches += 2
         return (gu, act, yp) if keep else (None, None, yp)
 
-    def moe_forward(self, i, h2, replay_ids=None, record=None, keep=False, residual=None, serving=False):
+    def _fp8_experts(self, xp, plan: MoeCtx, w1, w2):
+        """Both products of rows in expert order (bf16, or 8-bit rows) from the experts' 8-bit copies."""
+        from ..ops import fp8_block as F8
+
+        if not isinstance(xp, F8.Fp8Rows):
+            xp = F8.quantize_rows(xp)  # (rows past the live ones hold anything, and are not read)
+            self.launches += 1
+        act = F8.grouped_gated_linear(xp, self.mx[w1.data_ptr()], plan.tile_group, plan.num_tiles, self.status)
+        yp = F8.grouped_linear(act, self.mx[w2.data_ptr()], plan.tile_group, plan.num_tiles, status=self.status)
+        self.launches += 2 * self.C.fp8_grouped_launches(plan.max_rows, w1.shape[0])
+        return yp
+
+    def moe_forward(self, i, h2, replay_ids=None, record=None, keep=False, residual=None, serving=False, rows=None):
+        """``rows``: ``h2`` as 8-bit rows, for experts that are served from 8-bit copies."""
         cfg, P, C = self.cfg, self.store.params, self.C
         p = f"layers.{i}.moe."
         ids, w, probs = self._route(h2, P[p + "router.weight"], replay_ids, P.get(p + "router.bias"), serving)
@@ -348,13 +410,19 @@ class B200Qwen3:
             self.launches += 3
         if self.ep is not None:
             return self.ep.moe_forward(self, i, h2, ids, w, probs, keep, residual)
-        use_mx = bool(getattr(self, "mx", None)) and not keep and h2.shape[0] > 32
+        use_mx = bool(getattr(self, "mx", None)) and self.mx_kind != "fp8_block" and not keep and h2.shape[0] > 32
         plan = self._permute_plan(ids, cfg.num_experts, 64 if keep else (128 if use_mx else 1))
         plan.w, plan.probs = w, probs
-        xp = C.moe_permute(h2, plan.src, plan.num_tiles, cfg.moe_top_k)
-        if use_mx and self.mx_kind == "nvfp4":
-            plan.amax_in = C.absmax(h2.contiguous())  # the permuted rows hold exactly these values
-        gu, act, yp = self._experts_fwd(xp, plan, P[p + "w1"], P[p + "w2"], keep)
+        if rows is not None:
+            from ..ops.fp8_block import permute_rows
+
+            gu = act = xp = None
+            yp = self._fp8_experts(permute_rows(rows, plan.src, plan.num_tiles, cfg.moe_top_k), plan, P[p + "w1"], P[p + "w2"])
+        else:
+            xp = C.moe_permute(h2, plan.src, plan.num_tiles, cfg.moe_top_k)
+            if use_mx and self.mx_kind == "nvfp4":
+                plan.amax_in = C.absmax(h2.contiguous())  # the permuted rows hold exactly these values
+            gu, act, yp = self._experts_fwd(xp, plan, P[p + "w1"], P[p + "w2"], keep)
         y = C.moe_combine(yp, plan.dest, w, h2.shape[0], cfg.moe_top_k, residual)
         self.launches += 2
         saved = (plan, xp, gu, act, yp) if keep else None
@@ -443,11 +511,17 @@ class B200Qwen3:
         return dh2
 
     # ------------------------------------------------------------------ layer forward / backward
-    def _attn_qkv(self, i, x, positions, meta: Optional[InferMeta], kv_cache):
+    def _attn_qkv(self, i, x, positions, meta: Optional[InferMeta], kv_cache, fp8: bool = False):
         cfg, P, C = self.cfg, self.store.params, self.C
         p = f"layers.{i}."
-        h1, rstd1 = C.rmsnorm_fwd(x, None, P[p + "ln1.weight"], cfg.rms_eps)
-        qkv = self.linear(h1, P[p + "attn.qkv.weight"], serving=meta is not None)
+        if fp8:
+            from ..ops.fp8_block import rmsnorm_rows
+
+            h1, rstd1 = rmsnorm_rows(x, P[p + "ln1.weight"], cfg.rms_eps)[0], None
+            qkv = self._fp8_linear(h1, self.mx[P[p + "attn.qkv.weight"].data_ptr()])
+        else:
+            h1, rstd1 = C.rmsnorm_fwd(x, None, P[p + "ln1.weight"], cfg.rms_eps)
+            qkv = self.linear(h1, P[p + "attn.qkv.weight"], serving=meta is not None)
         if cfg.qkv_bias:
             qkv += P[p + "attn.qkv.bias"]
         kc = vc = slots = None
@@ -503,7 +577,8 @@ class B200Qwen3:
             y, _ = self.moe_forward(i, h2, replay_ids, record, keep=False, residual=x2, serving=True)
             return y
         serving = meta is not None
-        h1, rstd1, qkv, q, k, _, _ = self._attn_qkv(i, x, positions, meta, kv_cache)
+        fp8 = self._fp8_layer(i, x.shape[0])
+        h1, rstd1, qkv, q, k, _, _ = self._attn_qkv(i, x, positions, meta, kv_cache, fp8)
         scale = cfg.head_dim ** -0.5
         if meta is not None and not meta.is_prefill:
             att = torch.empty_like(q)
@@ -524,6 +599,8 @@ class B200Qwen3:
             self.launches += 2
         else:
             att, _ = self.attention(q, k, self._v_view(qkv), cu)
+        if fp8:
+            return self._mlp_fp8(i, att.view(att.shape[0], -1), x, replay_ids, record, serving)
         h2, _, x2 = self._o_proj_ln2(i, att.view(att.shape[0], -1), x, serving)
         if cfg.layer_is_moe(i):
             if (meta is not None and not meta.is_prefill and replay_ids is None and getattr(self.ep, "low_latency", False)
@@ -538,6 +615,22 @@ class B200Qwen3:
             self.launches += 2
             return yn.add_(x2)
         return self._row_parallel(act, P[p + "mlp.down.weight"], x2, serving)
+
+    def _mlp_fp8(self, i, att2, x, replay_ids, record, serving):
+        """What follows attention, from the weights' 8-bit copies: every product's input leaves the kernel before it in 8 bits."""
+        from ..ops.fp8_block import gated_linear, rmsnorm_rows
+
+        cfg, P = self.cfg, self.store.params
+        p = f"layers.{i}."
+        moe = cfg.layer_is_moe(i)
+        o = self._fp8_linear(att2, self.mx[P[p + "attn.o.weight"].data_ptr()])
+        rows, x2, h2 = rmsnorm_rows(o, P[p + "ln2.weight"], cfg.rms_eps, x, keep=moe)  # (the router reads bf16)
+        self.launches += 1
+        if moe:
+            return self.moe_forward(i, h2, replay_ids, record, keep=False, residual=x2, serving=serving, rows=rows)[0]
+        act = gated_linear(rows, self.mx[P[p + "mlp.gate_up.weight"].data_ptr()], self.status)
+        self.launches += 1
+        return self._fp8_linear(act, self.mx[P[p + "mlp.down.weight"].data_ptr()], x2)
 
     def _full_kv(self, prefix, k, v, kc, vc):
         """``PrefixInfo.full_kv`` in one launch for caches of the activations' type."""

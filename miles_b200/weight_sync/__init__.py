@@ -72,7 +72,7 @@ def sync_weights(actor, engines: Sequence, mode: str | None = None) -> dict:
     for e in engines:
         refresh = getattr(getattr(e, "model", None), "refresh_block_scaled", None)
         if refresh is not None:
-            refresh()  # engines that serve MXFP8 / NVFP4 copies re-quantise from the weights that just arrived
+            refresh()  # engines that serve quantised copies re-quantise from the weights that just arrived
     if actor.on_gpu:
         torch.cuda.synchronize()
     for p in pushers:
