@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "fp8_tile.cuh"
+#include "pdl.cuh"
 
 namespace mb {
 namespace {
@@ -168,6 +169,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot_s);
   cluster_sync_all();  // both CTAs' barriers and TMEM are there before either uses the other's
+  pdl_enter();
   const int total = tiles_of<GATED>(p);
   const int half_n = p.N / p.halves;
 
@@ -487,6 +489,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 __global__ void __launch_bounds__(1024)
 pair_tiles_kernel(const int* __restrict__ tile_group, const int* __restrict__ num_tiles, int max_tiles, int groups, int M, int4* __restrict__ out,
                   int* __restrict__ count) {
+  pdl_enter();
   __shared__ int run_s[32], taken_s[32];
   const int n = min(max(*num_tiles, 0), max_tiles), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const auto entry = [&](int i) {
@@ -624,10 +627,12 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.tile_group) {
     a.tiles = reinterpret_cast<const int4*>(g.workspace);
     a.num_tiles = static_cast<const int*>(g.workspace) + 4ll * g.max_tiles;
-    pair_tiles_kernel<<<1, 1024, 0, stream>>>(g.tile_group, g.num_tiles, g.max_tiles, g.groups, g.M, static_cast<int4*>(g.workspace),
-                                              static_cast<int*>(g.workspace) + 4ll * g.max_tiles);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fp8_fail(std::string("pair_tiles launch failed: ") + cudaGetErrorString(e));
+    const cudaError_t e = pdl_launch(pair_tiles_kernel, dim3(1), dim3(1024), 0, stream, g.tile_group, g.num_tiles, g.max_tiles, g.groups, g.M,
+                                     static_cast<int4*>(g.workspace), static_cast<int*>(g.workspace) + 4ll * g.max_tiles);
+    if (e != cudaSuccess) {
+      cudaGetLastError();  // (reported here)
+      return fp8_fail(std::string("pair_tiles launch failed: ") + cudaGetErrorString(e));
+    }
   }
   const long long m_tiles = g.tile_group ? g.max_tiles : (g.M + 2 * BM - 1) / (2 * BM);
   const int cols = GATED ? BN / 2 : BN;
@@ -638,13 +643,15 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
   if (e != cudaSuccess) {
     cudaGetLastError();  // (reported here)

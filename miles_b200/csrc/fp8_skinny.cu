@@ -3,13 +3,13 @@
 //
 // They are bound by the bytes of W, and by how many of them are on their way from how many SMs. So 128 rows of W are the tensor core's M and
 // the rows of x its N (16, 32, 64 or 128): no part of a tile is padding that has to be streamed. A block of 128 along K is one stage, one
-// buffer of TMEM and four tcgen05.mma; four warps add it to sums in registers, a row of W a thread, times the weights' scale and the scale
+// buffer of TMEM and four tcgen05.mma; warps add it to sums in registers, a row of W a thread, times the weights' scale and the scale
 // of each column's row of x, which a warp lays out in shared memory a block ahead. The blocks of a tile are shared by a cluster of up to
 // eight CTAs, whose sums meet in distributed shared memory in rank order, so results do not depend on timing. A gate-up weight's CTA
 // streams 128 gate rows and their 128 up rows, which are a whole block of silu(gate) * up: a warp finds its largest value by shuffles.
 //
 //   warp 0     : TMA producer (128-byte swizzle)          warp 1 : TMEM allocator, tcgen05.mma issuer
-//   warps 2..5 : TMEM -> sums in registers -> shared memory, cluster sum, store
+//   the others : four warps, or eight for 128 columns, TMEM -> sums in registers -> shared memory, cluster sum, store
 #include <cuda.h>
 #include <string.h>
 
@@ -21,7 +21,6 @@ namespace {
 
 constexpr int BM = 128, BK = 128;
 constexpr int W_BYTES = BM * BK;
-constexpr int THREADS = 192;
 constexpr int MAX_STAGES = 12;
 
 struct Args {
@@ -73,19 +72,22 @@ struct Shape {
   static constexpr int BUFS = NT * G <= 32 ? 4 : 2;
   static constexpr int TMEM = BUFS * NT * G;
   static constexpr int MIN_SMEM = TMEM * 228 * 2;  // TMEM / 512 of 228 KB
+  static constexpr int EPI_WARPS = NT * G >= 128 ? 8 : 4;  // (128 rows of x, us a block: four 0.69, eight 0.61)
+  static constexpr int COLS = NT * 4 / EPI_WARPS;     // rows of x that a warp sums up
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int STAGE = G * W_BYTES + NT * BK;
   static constexpr int PART = NT * BM * 4;         // a CTA's sums of one matrix, over the ring
 };
 
 template <int NT, bool GATED>
-__global__ void __launch_bounds__(THREADS, Shape<NT, GATED>::TMEM <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(Shape<NT, GATED>::THREADS, Shape<NT, GATED>::TMEM <= 128 ? 2 : 1)
 fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args p) {
   using S = Shape<NT, GATED>;
-  constexpr int G = S::G, BUFS = S::BUFS, STAGE = S::STAGE, PART = S::PART;
+  constexpr int G = S::G, BUFS = S::BUFS, STAGE = S::STAGE, PART = S::PART, COLS = S::COLS, EPI_WARPS = S::EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * BUFS];
-  __shared__ __align__(16) float scales_s[4][2][G * NT];  // of a warp's current block and the next
+  __shared__ __align__(16) float scales_s[EPI_WARPS][2][G * COLS];  // of a warp's current block and the next
   __shared__ uint32_t tmem_slot_s;
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
@@ -108,7 +110,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     }
     for (int b = 0; b < BUFS; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 4);
+      mbar_init(tempty_bar(b), EPI_WARPS);
     }
     fence_barrier_init();
     prefetch_tensormap(&map_w);
@@ -197,18 +199,18 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       }
       __syncwarp();
     } else {
-      const int quad = warp & 3;
-      constexpr int PER = NT >= 32 ? NT / 32 : 1;  // rows of x whose scales a lane fetches
+      const int quad = warp & 3, c0 = (warp - 2) / 4 * COLS;  // rows of W that this warp reaches in TMEM; its rows of x
+      constexpr int PER = COLS >= 32 ? COLS / 32 : 1;         // of which a lane fetches the scales of these
       const float* xs[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) xs[j] = p.xs + static_cast<long long>(min(t0 + min(lane + 32 * j, NT - 1), p.M - 1)) * p.blocks_k + kb0;
+      for (int j = 0; j < PER; ++j) xs[j] = p.xs + static_cast<long long>(min(t0 + c0 + min(lane + 32 * j, COLS - 1), p.M - 1)) * p.blocks_k + kb0;
       const float* ws0 = p.ws + (static_cast<long long>(group) * p.blocks_n + n0 / 128) * p.blocks_k + kb0;
       const float* ws1 = ws0 + (GATED ? static_cast<long long>(p.blocks_n / 2) * p.blocks_k : 0);
-      float acc[G][NT];
+      float acc[G][COLS];
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[g][i] = 0.f;
+        for (int i = 0; i < COLS; ++i) acc[g][i] = 0.f;
       float xn[PER], wn0 = 0.f, wn1 = 0.f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) xn[j] = 0.f;
@@ -219,13 +221,13 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         if (GATED) wn1 = ws1[0];
       }
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-      for (int b = 0; ok && b < blocks; ++b) {
+      for (int b = 0; b < blocks; ++b) {
         float* mine = scales_s[warp - 2][b & 1];
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-          if (NT >= 32 || lane < NT) {
+          if (COLS >= 32 || lane < COLS) {
             mine[lane + 32 * j] = xn[j] * wn0;
-            if (GATED) mine[NT + lane + 32 * j] = xn[j] * wn1;
+            if (GATED) mine[COLS + lane + 32 * j] = xn[j] * wn1;
           }
         __syncwarp();
         if (b + 1 < blocks) {
@@ -234,25 +236,26 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
           wn0 = ws0[b + 1];
           if (GATED) wn1 = ws1[b + 1];
         }
-        ok = f8::all_got(mbar_wait(tfull_bar(buf), tphase, abort_flag, p.status, ERR_WAIT_TMEM_FULL));
-        if (!ok) break;
+        // (a wait that runs out shows in `ok` at the end; what is read meanwhile is thrown away, and every later wait ends at once)
+        ok = mbar_wait(tfull_bar(buf), tphase, abort_flag, p.status, ERR_WAIT_TMEM_FULL) && ok;
+        __syncwarp();
         tc_fence_after();
-        constexpr int CH = NT >= 32 ? 32 : 16;
+        constexpr int CH = COLS >= 32 ? 32 : 16;
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int c = 0; c < NT; c += CH) {
+          for (int c = 0; c < COLS; c += CH) {
             uint32_t d[CH];
             if constexpr (CH == 32) {
-              tmem_ld_32x32(tmem + (buf * G + g) * NT + lanes + c, d);
+              tmem_ld_32x32(tmem + (buf * G + g) * NT + lanes + c0 + c, d);
               f8::tmem_ld_wait_for(d);
             } else {
-              tmem_ld_32x16(tmem + (buf * G + g) * NT + lanes + c, d);
+              tmem_ld_32x16(tmem + (buf * G + g) * NT + lanes + c0 + c, d);
               f8::tmem_ld_wait_for(d);
             }
 #pragma unroll
             for (int i = 0; i < CH; i += 4) {
-              const float4 s = *reinterpret_cast<const float4*>(mine + g * NT + c + i);
+              const float4 s = *reinterpret_cast<const float4*>(mine + g * COLS + c + i);
               acc[g][c + i] = fmaf(s.x, __uint_as_float(d[i]), acc[g][c + i]);
               acc[g][c + i + 1] = fmaf(s.y, __uint_as_float(d[i + 1]), acc[g][c + i + 1]);
               acc[g][c + i + 2] = fmaf(s.z, __uint_as_float(d[i + 2]), acc[g][c + i + 2]);
@@ -260,20 +263,19 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             }
           }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(buf));
+        if (lane == 0) mbar_arrive(tempty_bar(buf));  // (the wait for the loads was the whole warp's)
         if (++buf == BUFS) {
           buf = 0;
           tphase ^= 1u;
         }
       }
       // the sums of this CTA's blocks -> shared memory [matrix][row of x][row of W], over the ring: its last stage has been multiplied
-      if (ok) {
-        const uint32_t dst = base + (quad * 32 + lane) * 4;
+      if (f8::all_got(ok)) {
+        const uint32_t dst = base + c0 * (BM * 4) + (quad * 32 + lane) * 4;
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
+          for (int i = 0; i < COLS; ++i)
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + g * PART + i * (BM * 4)), "f"(acc[g][i]) : "memory");
       }
     }
@@ -282,7 +284,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     cluster_sync_all();
     if (warp >= 2) {
       const int n = n0 + lane * 4;
-      for (int t = static_cast<int>(rank) + static_cast<int>(ranks) * (warp - 2); t < count; t += static_cast<int>(ranks) * 4) {
+      for (int t = static_cast<int>(rank) + static_cast<int>(ranks) * (warp - 2); t < count; t += static_cast<int>(ranks) * EPI_WARPS) {
         float f[G][4];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -347,6 +349,27 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   }
 }
 
+// CTAs that share the blocks of a tile: while each keeps two and all that have rows are resident at once (by expert: at most a tile for
+// every row, and no more than the list has room for). Clusters of eight do not all find room at one CTA an SM: 128 rows, 2048 x 4096 16.2 us
+// against 10.7 for twice the rows in clusters of four.
+int split_of(const Fp8Gemm& g, long long z, int n_tiles, int blocks_k, int sms, int per_sm) {
+  const long long live = g.tile_group && g.M < z ? g.M : z;
+  const int resident = sms * per_sm;
+  int split = 1;
+  while (split < (per_sm == 1 ? 4 : 8) && live * n_tiles * split * 2 <= resident && blocks_k >= split * 2 * 2) split *= 2;
+  return split;
+}
+
+// Rows of x in a tile. Experts are not equally liked: half as many again as the average fit, four times as many where the average is four at most
+// (gate-up experts of 64 tokens 69 us, with tiles of 32 rows 75).
+int rows_of_tile(const Fp8Gemm& g) {
+  if (!g.tile_group) return g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 || g.q ? 64 : 128;
+  const long long live = g.groups < g.M ? g.groups : g.M;
+  if (g.M <= 4 * live) return 16;
+  const long long rows = (g.M + g.M / 2) / live;
+  return rows <= 32 ? 32 : rows <= 64 || g.q ? 64 : 128;
+}
+
 template <int NT, bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
   using S = Shape<NT, GATED>;
@@ -383,12 +406,7 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   a.status = g.status;
   const int n_tiles = (g.N / S::G + BM - 1) / BM;
   const long long z = g.tile_group ? g.max_tiles : (g.M + NT - 1) / NT;
-  // Row tiles that hold rows: at most one of an expert for every row, and no more than the list has room for.
-  const long long live = g.tile_group ? (g.M < z ? g.M : z) : z;
-  // The blocks are split while every CTA keeps two and all CTAs are resident at once.
-  const int resident = sms * (S::TMEM <= 128 ? 2 : 1);
-  int split = 1;
-  while (split < 8 && live * n_tiles * split * 2 <= resident && a.blocks_k >= split * 2 * 2) split *= 2;
+  const int split = split_of(g, z, n_tiles, a.blocks_k, sms, S::TMEM <= 128 ? 2 : 1);
   a.per_rank = (a.blocks_k + split - 1) / split;
   int stages = (MOST - 1024) / S::STAGE;
   if (stages > MAX_STAGES) stages = MAX_STAGES;
@@ -402,7 +420,7 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   if (n_tiles > 65535 || z > 65535) return fp8_fail("too many tiles");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, n_tiles, static_cast<unsigned>(z));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -424,12 +442,30 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
 
 }  // namespace
 
-// Rows by expert: few for each expert on average, as many as its list may hold. Otherwise while pairs' tiles would leave the GPU idle.
+// Few rows, or few tiles: by what either kernel costs, us. Pairs (fp8_gemm.cu) take 4.5 us and, for each round of their tiles over the SMs, 0.48 a
+// block of 128 along K and 1.2 at its end (2.5 with SwiGLU; by expert 2 more to join row tiles). The CTAs here take 5.7 and, a round, 0.61 to
+// 0.75 a block where one fits an SM; where two do, 3 and 3 a round, and 0.45 a block; or what the blocks of all of them need to arrive.
+// Measured, us, pairs / here: 24576 x 4096 gate-up, 64 rows 42 / 31, 128 rows 42 / 58; 6144 x 4096, 128 rows 21 / 16, 512 22 / 52; 4096 x 12288, 256
+// rows 50 / 36, 512 50 / 66; 128 experts, gate-up 1536 x 2048, 16 rows each 125 / 83, 64 127 / 151, 2048 x 768, 16 rows 66 / 58, 48 71 / 118.
 bool fp8_is_skinny(const Fp8Gemm& g) {
-  if (g.tile_group) return g.M <= 48ll * g.groups && g.max_tiles <= 65535;
-  const int cols = g.q ? 128 : 256;
-  const long long pairs = static_cast<long long>((g.M + 255) / 256) * ((g.N / (g.q ? 2 : 1) + cols - 1) / cols);
-  return g.M <= 128 || pairs < 60;
+  if (g.M <= 0) return true;
+  int sms = 0;
+  fp8_device(&sms);
+  const int G = g.q ? 2 : 1, n = g.N / G, blocks_k = (g.K + BK - 1) / BK, nt = rows_of_tile(g);
+  const long long live = g.M < g.groups ? g.M : g.groups;  // experts with rows
+  if (g.tile_group && (g.M > live * 2 * nt / 3 || g.max_tiles > 65535)) return false;  // (more rows than such tiles hold)
+  const long long pairs = (g.tile_group ? live + g.M / 256 : (g.M + 255) / 256) * ((n + 256 / G - 1) / (256 / G));
+  const long long z = g.tile_group ? live : (g.M + nt - 1) / nt;
+  const int n_tiles = (n + BM - 1) / BM, per_sm = nt * G < 128 ? 2 : 1, resident = sms * per_sm;
+  if (z > 65535 || n_tiles > 65535) return false;
+  const int split = split_of(g, z, n_tiles, blocks_k, sms, per_sm);
+  const long long ctas = z * n_tiles * split;
+  const double arrive = static_cast<double>(ctas < resident ? ctas : resident) * G * W_BYTES / 6.0e6;
+  const double alone = nt * G < 128 ? 0.45 : G == 2 ? 0.75 : 0.61, block = arrive > alone ? arrive : alone;
+  const double rounds = static_cast<double>((ctas + resident - 1) / resident), own = (blocks_k + split - 1) / split * block;
+  const double here = per_sm == 1 ? rounds * (5.7 + own) : 3.0 + rounds * (3.0 + own);
+  const double there = (g.tile_group ? 6.5 : 4.5) + static_cast<double>((2 * pairs + sms - 1) / sms) * (0.48 * blocks_k + (G == 2 ? 2.5 : 1.2));
+  return here <= there;
 }
 
 int fp8_grouped_launches(long long rows, int groups) {
@@ -442,12 +478,11 @@ int fp8_grouped_launches(long long rows, int groups) {
 }
 
 int fp8_skinny_launch(const Fp8Gemm& g, cudaStream_t stream) {
-  const long long rows = g.tile_group ? g.M / (g.groups < g.M ? g.groups : g.M) : g.M;  // of a tile, or an expert's on average
-  if (g.q) return rows <= 16 ? launch<16, true>(g, stream) : rows <= 32 ? launch<32, true>(g, stream) : launch<64, true>(g, stream);
-  if (rows <= 16) return launch<16, false>(g, stream);
-  if (rows <= 32) return launch<32, false>(g, stream);
-  if (rows <= 64) return launch<64, false>(g, stream);
-  return launch<128, false>(g, stream);
+  const int nt = rows_of_tile(g);
+  if (g.q) return nt == 16 ? launch<16, true>(g, stream) : nt == 32 ? launch<32, true>(g, stream) : launch<64, true>(g, stream);
+  if (nt == 16) return launch<16, false>(g, stream);
+  if (nt == 32) return launch<32, false>(g, stream);
+  return nt == 64 ? launch<64, false>(g, stream) : launch<128, false>(g, stream);
 }
 
 }  // namespace mb
