@@ -320,6 +320,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const Tile tl = tile_at<GATED>(p, t);
       const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
       const int rows = min(max(tl.row_end - row0, 0), 32);
+      if (!GATED && p.residual && lane < rows && n0 + part * COLS < p.N)  // on its way into L2 while the sums are formed
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + static_cast<long long>(row0 + lane) * p.ldr + n0 + part * COLS));
       float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
@@ -577,8 +579,12 @@ int fp8_device(int* sms) {
   cudaGetDevice(&dev);
   int n = known[dev & 63].load(std::memory_order_relaxed);
   if (n == 0) {
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    known[dev & 63].store(n, std::memory_order_relaxed);
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) {
+      known[dev & 63].store(n, std::memory_order_relaxed);
+    } else {  // (no device: what is asked then is only which kernel would run)
+      cudaGetLastError();
+      n = 148;
+    }
   }
   *sms = n;
   return dev;
