@@ -8,6 +8,9 @@
 // eight CTAs, whose sums meet in distributed shared memory in rank order, so results do not depend on timing. A gate-up weight's CTA
 // streams 128 gate rows and their 128 up rows, which are a whole block of silu(gate) * up: a warp finds its largest value by shuffles.
 //
+// Measured, us (the bytes of W alone at 6.5 TB/s): one row 5120 x 2048 5.3 (1.6), 23 rows 2560 x 9728 9.3 (3.8), 64 rows 6144 x 4096 11.3 (3.9);
+// 128 experts, 64 tokens by eight: gate-up 1536 x 2048 70 (61).
+//
 //   warp 0     : TMA producer (128-byte swizzle)          warp 1 : TMEM allocator, tcgen05.mma issuer
 //   the others : four warps, or eight for 128 columns, TMEM -> sums in registers -> shared memory, cluster sum, store
 #include <cuda.h>

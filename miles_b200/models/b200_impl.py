@@ -227,8 +227,8 @@ class B200Qwen3:
         return len(self.mx)
 
     def _fp8(self, w, rows: int):
-        """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None. us, one dense layer's products with their norms and
-        activation, bf16 / 8 bits: see DECODE."""
+        """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None: up to ``SMALL_T`` rows the fused kernels on bf16 weights take fewer
+        launches. us a layer, bf16 / 8 bits: a mixture's decode steps of 16 rows 187 / 138, of 64 292 / 206; a dense layer of 16 rows 114 / 78."""
         mx = getattr(self, "mx", None)
         return mx.get(w.data_ptr()) if mx and self.mx_kind == "fp8_block" and rows > self.SMALL_T else None
 

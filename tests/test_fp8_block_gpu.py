@@ -213,6 +213,46 @@ def test_linear_of_no_rows_and_bf16_rows(F8):
     assert torch.equal(F8.linear(x, w), F8.linear(F8.quantize_rows(x), w))
 
 
+def test_offsets_beyond_32_bits(F8):
+    """Rows, results and weights whose places pass 2^31 elements: the last ones are right, and so are the first."""
+    g = gen(8)
+    T, N = 270000, 8192
+    x = F8.quantize_rows(torch.randn(T, 128, generator=g, device=DEV).bfloat16())
+    w = F8.quantize_weight(torch.randn(N, 128, generator=g, device=DEV).bfloat16())
+    y = F8.linear(x, w)
+    for rows in (slice(0, 60), slice(T - 60, T)):
+        part = F8.Fp8Rows(x.q[rows], x.scales[rows])
+        check_bf16(y[rows], *product64(part, w))
+    r = F8.quantize_rows(y)
+    normed, _, _ = F8.rmsnorm_rows(y, torch.ones(N, device=DEV).bfloat16(), 1e-6)
+    for rows in (slice(0, 20), slice(T - 20, T)):
+        check_rows(F8.Fp8Rows(r.q[rows], r.scales[rows]), y[rows].double())
+        h = y[rows].double()
+        want = h / (h.square().mean(1, keepdim=True) + 1e-6).sqrt()
+        check_rows(F8.Fp8Rows(normed.q[rows], normed.scales[rows]), want, 45 * 2.0 ** -24 * want.abs())
+    del y, r, normed
+    E, N, K = 260, 2048, 4096  # 2.2 GB of weights
+    q = torch.randint(0, 120, (E, N, K), generator=g, device=DEV, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    w = F8.Fp8Weight(q, torch.rand(E, N // 128, K // 128, generator=g, device=DEV))
+    for count in (3, 140):  # by either kernel
+        x = F8.quantize_rows(acts(count * E, K, g))
+        tiles = torch.tensor(tiles_of([count] * E), dtype=torch.int32, device=DEV)
+        y = F8.grouped_linear(x, w, tiles, torch.tensor([len(tiles)], dtype=torch.int32, device=DEV))
+        for e in (0, E - 1):
+            rows = slice(e * count, (e + 1) * count)
+            check_bf16(y[rows], *product64(F8.Fp8Rows(x.q[rows], x.scales[rows]), F8.Fp8Weight(w.q[e], w.scales[e])))
+
+
+@pytest.mark.parametrize("T", [6, 300])
+def test_the_status_word_is_left_alone(F8, T):
+    """A code that another kernel left stays for the model to report."""
+    g = gen(T)
+    w = F8.quantize_weight(torch.randn(384, 256, generator=g, device=DEV).bfloat16(), 2)
+    status = torch.full((1,), 17, dtype=torch.int32, device=DEV)
+    F8.gated_linear(acts(T, 256, g), w, status)
+    assert int(status) == 17
+
+
 def test_linear_keeps_nan_and_infinities_in_their_rows(F8):
     g = gen(3)
     for T in (20, 200):
@@ -379,6 +419,23 @@ def test_captured_and_on_other_streams(F8, ext, T):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got_b + got_c, want_b + want_c))
     assert int(b["status"]) == int(c["status"]) == 0
+
+
+def test_refusals_of_operands_on_the_device(F8):
+    x, w = F8.quantize_rows(acts(4, 256, gen(1))), F8.quantize_weight(torch.randn(64, 256, device=DEV).bfloat16())
+    wide = torch.zeros(4 * 256 + 64, dtype=torch.uint8, device=DEV)
+    off = lambda n: wide[n:n + 1024].view(torch.float8_e4m3fn).view(4, 256)  # noqa: E731
+    for call, words in ((lambda: F8.linear(F8.Fp8Rows(off(8), x.scales), w), "16-byte aligned"),
+                        (lambda: F8.linear(F8.Fp8Rows(x.q, x.scales.cpu()), w), "on the device"),
+                        (lambda: F8.linear(x, w, acts(4, 63, gen(2))), "residual must be"),
+                        (lambda: F8.linear(x, w, out=torch.empty(4, 64, device=DEV)), "out must be"),
+                        (lambda: F8.linear(x, w, out=torch.empty(1, 64, device=DEV).bfloat16().expand(4, 64)), "overlap"),
+                        (lambda: F8.quantize_rows(acts(4, 264, gen(3))[:, 4:260]), "16-byte aligned"),
+                        (lambda: F8.rmsnorm_rows(acts(4, 256, gen(4)), torch.ones(256, device=DEV).bfloat16(), 1e-6, acts(4, 260, gen(5))[:, :256]), "16-byte aligned"),
+                        (lambda: F8.gated_linear(x, F8.quantize_weight(torch.randn(96, 256, device=DEV).bfloat16())), "gate-up weight")):
+        with pytest.raises(RuntimeError, match=words):
+            call()
+    assert F8.linear(x, w).isfinite().all()  # (a refused call leaves nothing behind)
 
 
 # ------------------------------------------------------------------------------------------------ weights
