@@ -416,6 +416,11 @@ class Engine:
         self.weight_version = self.weight_version + 1 if version is None else int(version)
         return self.weight_version
 
+    def weights_arrived(self) -> None:
+        """Weights changed in place: an engine that serves from 8-bit copies (``fp8_block``) quantises them anew, where captured steps read them."""
+        if getattr(self.model, "mx_kind", None) == "fp8_block":
+            self.model.refresh_block_scaled()
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self.prefilling or self._pending is not None)
 

@@ -91,6 +91,7 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
             dst.copy_(tensor.to(dst.dtype))
             n += 1
         if body.get("weight_version") is not None:
+            engine.weights_arrived()
             engine.update_weight_version(body["weight_version"])
         return {"success": True, "num_tensors": n}
 
@@ -100,6 +101,7 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
         from ..checkpoint import load_hf
 
         n = load_hf(engine.cfg, engine.store, body["model_path"], strict=False)
+        engine.weights_arrived()
         if body.get("weight_version") is not None:
             engine.update_weight_version(body["weight_version"])
         return {"success": True, "num_tensors": n}
@@ -107,6 +109,7 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
     @app.post("/update_weight_version")
     async def update_weight_version(req: Request):
         body = await req.json()
+        engine.weights_arrived()  # (buckets may have come without a version of their own)
         return {"weight_version": engine.update_weight_version(body.get("new_version", body.get("weight_version")))}
 
     @app.post("/end_weight_update")

@@ -33,6 +33,7 @@ def register_extra(app, engine, state: dict) -> None:
 
         n = await asyncio.to_thread(receive_bucket, b, engine.store)
         if b.get("weight_version") is not None:
+            engine.weights_arrived()
             engine.update_weight_version(b["weight_version"])
         return {"success": True, "num_tensors": n}
 
@@ -43,6 +44,7 @@ def register_extra(app, engine, state: dict) -> None:
         from ..weight_sync.disk_delta import apply_delta_dir
 
         n = await asyncio.to_thread(apply_delta_dir, engine.store, b["path"])
+        engine.weights_arrived()
         if b.get("weight_version") is not None:
             engine.update_weight_version(b["weight_version"])
         return {"success": True, "num_tensors": n}
@@ -79,6 +81,7 @@ def register_extra(app, engine, state: dict) -> None:
         tensors = dict(take_bucket(b["bucket_id"]))
         scale = float(b.get("scaling", 1.0))
         merge_adapter_into(engine.store, tensors, scale)
+        engine.weights_arrived()
         state["adapters"][name] = (tensors, scale)
         return {"success": True, "loaded_adapters": sorted(state["adapters"])}
 
@@ -91,6 +94,7 @@ def register_extra(app, engine, state: dict) -> None:
         if ad is None:
             raise HTTPException(404, f"adapter {b['lora_name']!r} is not loaded")
         merge_adapter_into(engine.store, ad[0], -ad[1])
+        engine.weights_arrived()
         return {"success": True, "loaded_adapters": sorted(state["adapters"])}
 
     # ------------------------------------------------------------------ profiling
