@@ -18,7 +18,11 @@
 //
 //   warp 0      : TMA producer (128-byte swizzle)          warp 1 : TMEM allocator, tcgen05.mma issuer
 //   warps 2, 3  : scales of the rows times the weights', eight blocks ahead
-//   warps 4..19 : sums in registers, a row and 64 columns a thread, then rows of 64 bytes through shared memory
+//   warps 4..19 : sums in registers, a row and 64 columns a thread, then rows through shared memory
+//
+// y leaves in boxes of 32 rows x 64 columns by asynchronous stores that nobody waits for until the warp's next box (their 32 KB more take a stage of
+// operands; with stores by threads, from half of that: 87 -> 73 us at 32768 x 2048 x 768, 129 -> 118 at K = 1536, 146 -> 143 at 8192 x 2048 x
+// 8192). An expert's last rows, with another's behind them in the box, and rows of y that are not 16 bytes apart are stored by threads.
 //
 // Measured, us: 8192 x 24576 x 4096 gate-up 975 (1690 TFLOP/s), 8192 x 4096 x 4096 with residual 180, experts of 65536 rows, 128 of 1536 x
 // 2048 gate-up 360, 2048 x 768 226.
@@ -39,14 +43,19 @@ namespace {
 
 constexpr int BM = 128, BN = 256, BK = 128;  // rows of a CTA, columns of its pair's tile (W rows), columns of a block
 constexpr int COLS = 64;                     // of a thread
-constexpr int STAGES = 5, BUFS = 2;
+constexpr int BUFS = 2;
 constexpr int X_BYTES = BM * BK, W_BYTES = BN / 2 * BK;  // of a stage: this CTA's rows of x, and of W
 constexpr int STAGE = X_BYTES + W_BYTES;
 constexpr int EPI_WARPS = 16;
 constexpr int THREADS = 128 + 32 * EPI_WARPS;  // the first warpgroup gives registers to the others, which sum up
-constexpr int STAGING = EPI_WARPS * 2048;
 constexpr int AHEAD = 8, SLOTS = 2;          // blocks of scales in a slot
 constexpr int SLOT_BYTES = 2 * AHEAD * BM * 4;
+// Stages, and what a warp has to stage its 32 rows: whole rows of y leave by asynchronous stores, which the next tile need not wait for.
+template <bool GATED>
+struct Room {
+  static constexpr int STAGES = GATED ? 5 : 4, WARP = GATED ? 2048 : 4096;
+  static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * WARP + SLOTS * SLOT_BYTES + 1024;
+};
 
 struct Args {
   int M, N, K;
@@ -128,11 +137,12 @@ __device__ __forceinline__ Tile tile_at(const Args& p, int t) {
 
 template <bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args p) {
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y, const Args p) {
+  constexpr int STAGES = Room<GATED>::STAGES, WARP = Room<GATED>::WARP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = base + STAGES * STAGE;
-  const uint32_t scales = staging + STAGING;
+  const uint32_t scales = staging + EPI_WARPS * WARP;
   __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFS + 2 * SLOTS + 1];
   __shared__ uint32_t tmem_slot_s;
   __shared__ int abort_s;
@@ -306,7 +316,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // rows of the tile that this warp reaches in TMEM; its part of the columns: 64 of y, or 32 of the gates and 32 of their up columns
     const int quad = warp & 3, part = (warp - 4) >> 2, half = part >> 1;
-    const uint32_t mine = staging + (warp - 4) * 2048;
+    const uint32_t mine = staging + (warp - 4) * WARP;
     const uint32_t from0 = tmem + (GATED ? half * (BN / 2) + (part & 1) * 32 : part * COLS) + (static_cast<uint32_t>(quad * 32) << 16);
     constexpr int THEN = GATED ? BN / 4 : 32;  // from its first 32 columns to the others
     const uint32_t my_scales = scales + (GATED ? 0 : half * (SLOT_BYTES / 2)) + (quad * 32 + lane) * 4;
@@ -393,7 +403,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll
         for (int k = 1; k < 4; ++k) {
           float other;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((part ^ k) * 4 + quad) * 2048 + there) : "memory");
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(staging + ((part ^ k) * 4 + quad) * WARP + there) : "memory");
           amax = f8::max_nan(amax, other);
         }
         const float s = f8::scale_of(amax);
@@ -417,68 +427,81 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         __syncwarp();
       } else {
+        // what this warp staged last has been read
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+        // rows of 128 bytes, 16-byte pieces in places that differ by row (the swizzle of the tensor map)
+        const auto place = [&](int r, int piece) { return mine + r * 128 + ((piece ^ (r & 7)) * 16); };
+        const int c0 = n0 + part * COLS;
+        if (p.residual) {  // joins the sums before they are rounded; read in whole rows, 32 columns at a time
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {  // 32 columns at a time: rows of 64 bytes, 16-byte pieces in places that differ by row
-          const int c0 = n0 + part * COLS + j * 32;
-          if (c0 >= p.N) break;
-          const auto place = [&](int r, int piece) { return mine + r * 64 + ((piece ^ ((r >> 1) & 3)) * 16); };
-          const auto element = [&](int r) { return place(r, lane >> 3) + (lane & 7) * 2; };
-          const int r8 = lane >> 2, piece = lane & 3;  // whole rows: eight at a time, four lanes each
-          if (p.residual) {                            // joins the sums before they are rounded: read in whole rows, too
-            if (p.vec_r && c0 + 32 <= p.N) {
+          for (int j = 0; j < 2; ++j) {
+            const int c = c0 + 32 * j;
+            if (p.vec_r && c + 32 <= p.N) {
+              const int r8 = lane >> 2, piece = lane & 3;
               uint4 v[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                v[i] = 8 * i + r8 < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + 8 * i + r8) * p.ldr + c0 + piece * 8)
+                v[i] = 8 * i + r8 < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + 8 * i + r8) * p.ldr + c + piece * 8)
                                          : make_uint4(0, 0, 0, 0);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) st_shared(place(8 * i + r8, piece), v[i]);
+              for (int i = 0; i < 4; ++i) st_shared(place(8 * i + r8, 4 * j + piece), v[i]);
             } else {
 #pragma unroll 4
               for (int r = 0; r < 32; ++r) {
                 unsigned short v = 0;
-                if (r < rows && c0 + lane < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c0 + lane];
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r)), "h"(v) : "memory");
-              }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 v = ld_shared(place(lane, i));
-              const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 f = __bfloat1622float2(b[k]);
-                acc[32 * j + 8 * i + 2 * k] += f.x;
-                acc[32 * j + 8 * i + 2 * k + 1] += f.y;
+                if (r < rows && c + lane < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c + lane];
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(place(r, 4 * j + (lane >> 3)) + (lane & 7) * 2), "h"(v) : "memory");
               }
             }
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* f = acc + 32 * j + 8 * i;
-            st_shared(place(lane, i), make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
-          }
           __syncwarp();
-          if (p.vec_y && c0 + 32 <= p.N) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * i + r8;
-              const uint4 v = ld_shared(place(r, piece));
-              if (r < rows) *reinterpret_cast<uint4*>(p.y + static_cast<long long>(row0 + r) * p.ldy + c0 + piece * 8) = v;
-            }
-          } else {
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-              unsigned short v;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(element(r)) : "memory");
-              if (r < rows && c0 + lane < p.N) reinterpret_cast<unsigned short*>(p.y)[static_cast<long long>(row0 + r) * p.ldy + c0 + lane] = v;
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = ld_shared(place(lane, i));
+            const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __bfloat1622float2(b[k]);
+              acc[8 * i + 2 * k] += f.x;
+              acc[8 * i + 2 * k + 1] += f.y;
             }
           }
-          __syncwarp();
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float* f = acc + 8 * i;
+          st_shared(place(lane, i), make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
+        }
+        // All 32 rows are of this tile, or the rows of y end with it: the store leaves out what lies outside y.
+        if (p.vec_y && (rows == 32 || row0 + rows == p.M)) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0 && rows > 0 && c0 < p.N) {
+            tma_store_2d(&map_y, mine, c0, row0);
+            tma_store_commit();
+          }
+        } else if (p.vec_y && c0 + COLS <= p.N) {  // the last rows of an expert's, with another's behind them
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3), piece = lane & 7;
+            if (r < rows) *reinterpret_cast<uint4*>(p.y + static_cast<long long>(row0 + r) * p.ldy + c0 + piece * 8) = ld_shared(place(r, piece));
+          }
+        } else {
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 64; ++i) {
+            const int r = i >> 1, c = (i & 1) * 32 + lane;
+            unsigned short v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(place(r, c >> 3) + (c & 7) * 2) : "memory");
+            if (r < rows && c0 + c < p.N) reinterpret_cast<unsigned short*>(p.y)[static_cast<long long>(row0 + r) * p.ldy + c0 + c] = v;
+          }
+        }
+        __syncwarp();
       }
     }
+    if (!GATED && lane == 0) tma_store_wait<0>();  // shared memory outlives the stores
   }
 
   tc_fence_before();
@@ -578,6 +601,18 @@ int fp8_make_map(CUtensorMap* map, const void* ptr, long long rows, long long co
   return 0;
 }
 
+// bf16 matrix [rows, cols] that boxes of 32 rows x 64 columns are stored to
+static int fp8_make_out_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[2] = {64u, 32u};
+  const cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fp8_fail("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
+  return 0;
+}
+
 int fp8_device(int* sms) {
   static std::atomic<int> known[64];
   int dev = 0;
@@ -614,7 +649,7 @@ Args args_of(const Fp8Gemm& g) {
   a.ldy = g.ldy;
   a.residual = static_cast<const __nv_bfloat16*>(g.residual);
   a.ldr = g.ldr;
-  a.vec_y = g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+  a.vec_y = !g.q && g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
   a.vec_r = g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0;
   a.vec_s = a.blocks_k % 4 == 0 && (reinterpret_cast<uintptr_t>(g.xs) & 15) == 0;
   a.q = g.q;
@@ -625,8 +660,8 @@ Args args_of(const Fp8Gemm& g) {
 
 template <bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
-  constexpr int SMEM = STAGES * STAGE + STAGING + SLOTS * SLOT_BYTES + 1024;
-  CUtensorMap mx, mw;
+  constexpr int SMEM = Room<GATED>::SMEM;
+  CUtensorMap mx, mw, my;
   if (fp8_make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
   if (fp8_make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, GATED ? 64 : 128)) return -1;
   int sms = 0;
@@ -635,6 +670,8 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   auto kernel = fp8_gemm_kernel<GATED>;
   if (fp8_allow_smem(kernel, SMEM, asked, dev)) return -1;
   Args a = args_of(g);
+  memset(&my, 0, sizeof(my));
+  if (a.vec_y && fp8_make_out_map(&my, g.y, g.M, g.N, g.ldy)) return -1;
   if (g.tile_group) {
     a.tiles = reinterpret_cast<const int4*>(g.workspace);
     a.num_tiles = static_cast<const int*>(g.workspace) + 4ll * g.max_tiles;
@@ -663,7 +700,7 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, a);
   if (e != cudaSuccess) {
     cudaGetLastError();  // (reported here)
     return fp8_fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));

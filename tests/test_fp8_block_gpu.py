@@ -206,6 +206,26 @@ def test_linear_operands_apart(F8, T, N):
     assert torch.equal(F8.linear(x, w, y, out=y), F8.linear(x, w, res))
 
 
+@pytest.mark.parametrize("T", [257, 300, 511])
+@pytest.mark.parametrize("N", [8, 200, 264, 1001])
+def test_linear_into_part_of_a_wide_result(F8, T, N):
+    """The last rows and columns end inside a box of 32 x 64 that leaves at once; what lies around the result stays."""
+    g = gen(T + N)
+    x, w = F8.quantize_rows(acts(T, 400, g)), F8.quantize_weight(torch.randn(N, 400, generator=g, device=DEV).bfloat16())
+    want, err = product64(x, w)
+    pad = -N % 8
+    for residual in (False, True):
+        buf = torch.full((T + 40, N + pad + 80), 7.0, device=DEV).bfloat16()
+        res = acts(T, N, g) if residual else None
+        got = F8.linear(x, w, res, out=buf[3:3 + T, 16:16 + N])
+        if residual:
+            check_bf16(got, want + res.double(), err + 2.0 ** -23 * (want.abs() + res.double().abs()))
+        else:
+            check_bf16(got, want, err)
+        buf[3:3 + T, 16:16 + N] = 7.0
+        assert (buf == 7).all()
+
+
 def test_linear_of_no_rows_and_bf16_rows(F8):
     w = F8.quantize_weight(torch.randn(64, 128, device=DEV).bfloat16())
     assert F8.linear(F8.quantize_rows(torch.zeros(0, 128, device=DEV).bfloat16()), w).shape == (0, 64)
