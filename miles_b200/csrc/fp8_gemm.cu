@@ -137,13 +137,14 @@ __device__ __forceinline__ Tile tile_at(const Args& p, int t) {
 
 template <bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y, const Args p) {
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
+                const __grid_constant__ CUtensorMap map_r, const Args p) {
   constexpr int STAGES = Room<GATED>::STAGES, WARP = Room<GATED>::WARP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = base + STAGES * STAGE;
   const uint32_t scales = staging + EPI_WARPS * WARP;
-  __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFS + 2 * SLOTS + 1];
+  __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFS + 2 * SLOTS + 1 + EPI_WARPS];
   __shared__ uint32_t tmem_slot_s;
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
@@ -174,6 +175,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       mbar_init(sempty_bar(s), EPI_WARPS);
     }
     mbar_init(amax_bar, 32 * EPI_WARPS);
+    for (int w = 0; w < EPI_WARPS; ++w) mbar_init(amax_bar + 8u + 8u * w, 1);
     fence_barrier_init();
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
@@ -329,14 +331,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       if (lane == 0) f8::arrive_relaxed(tempty0 + 8u * buf);
     };
     int buf = 0, slot = 0, tiles_done = 0;
-    uint32_t tphase = 0, sphase = 0;
+    uint32_t tphase = 0, sphase = 0, rphase = 0;
+    const uint32_t residual_bar = amax_bar + 8u + 8u * (warp - 4);
     bool ok = true;
     for (int t = first_tile; t < total; t += step, ++tiles_done) {
       const Tile tl = tile_at<GATED>(p, t);
       const int row0 = tl.row0 + rank * BM + quad * 32, n0 = tl.n0;  // this warp's rows
       const int rows = min(max(tl.row_end - row0, 0), 32);
-      if (!GATED && p.residual && lane < rows && n0 + part * COLS < p.N)  // on its way into L2 while the sums are formed
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + static_cast<long long>(row0 + lane) * p.ldr + n0 + part * COLS));
+      const bool ahead = !GATED && p.residual && p.vec_r && rows > 0 && n0 + part * COLS < p.N;
+      if (ahead) {  // the residual's box arrives while the sums are formed
+        fence_proxy_async();  // (what threads read here for the last tile)
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_wait_read<0>();
+          mbar_expect_tx(residual_bar, WARP);
+          tma_load_2d(mine, &map_r, residual_bar, n0 + part * COLS, row0);
+        }
+        __syncwarp();
+      }
       float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
@@ -427,32 +439,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         __syncwarp();
       } else {
-        // what this warp staged last has been read
-        if (lane == 0) tma_store_wait_read<0>();
-        __syncwarp();
-        // rows of 128 bytes, 16-byte pieces in places that differ by row (the swizzle of the tensor map)
+        // rows of 128 bytes, 16-byte pieces in places that differ by row (the swizzle of the tensor maps)
         const auto place = [&](int r, int piece) { return mine + r * 128 + ((piece ^ (r & 7)) * 16); };
         const int c0 = n0 + part * COLS;
-        if (p.residual) {  // joins the sums before they are rounded; read in whole rows, 32 columns at a time
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int c = c0 + 32 * j;
-            if (p.vec_r && c + 32 <= p.N) {
-              const int r8 = lane >> 2, piece = lane & 3;
-              uint4 v[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[i] = 8 * i + r8 < rows ? *reinterpret_cast<const uint4*>(p.residual + static_cast<long long>(row0 + 8 * i + r8) * p.ldr + c + piece * 8)
-                                         : make_uint4(0, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) st_shared(place(8 * i + r8, 4 * j + piece), v[i]);
-            } else {
+        if (ahead) {
+          ok = f8::all_got(mbar_wait(residual_bar, rphase, abort_flag, p.status, ERR_WAIT_FULL));
+          if (!ok) break;
+          rphase ^= 1u;
+        } else {  // what this warp staged last has been read
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        }
+        if (p.residual) {  // joins the sums before they are rounded
+          if (!ahead) {
 #pragma unroll 4
-              for (int r = 0; r < 32; ++r) {
-                unsigned short v = 0;
-                if (r < rows && c + lane < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c + lane];
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(place(r, 4 * j + (lane >> 3)) + (lane & 7) * 2), "h"(v) : "memory");
-              }
+            for (int i = 0; i < 64; ++i) {
+              const int r = i >> 1, c = (i & 1) * 32 + lane;
+              unsigned short v = 0;
+              if (r < rows && c0 + c < p.N) v = reinterpret_cast<const unsigned short*>(p.residual)[static_cast<long long>(row0 + r) * p.ldr + c0 + c];
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(place(r, c >> 3) + (c & 7) * 2), "h"(v) : "memory");
             }
           }
           __syncwarp();
@@ -501,7 +506,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         __syncwarp();
       }
     }
-    if (!GATED && lane == 0) tma_store_wait<0>();  // shared memory outlives the stores
+    if (!GATED && lane == 0) {  // shared memory outlives the stores, and where a wait has run out, the residual's box has a bounded time to land
+      tma_store_wait<0>();
+      if (!ok && p.residual) {
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) {
+        }
+      }
+    }
   }
 
   tc_fence_before();
@@ -601,8 +613,8 @@ int fp8_make_map(CUtensorMap* map, const void* ptr, long long rows, long long co
   return 0;
 }
 
-// bf16 matrix [rows, cols] that boxes of 32 rows x 64 columns are stored to
-static int fp8_make_out_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld) {
+// bf16 matrix [rows, cols] that boxes of 32 rows x 64 columns are stored to or read from
+static int fp8_make_bf16_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
   const cuuint32_t box[2] = {64u, 32u};
@@ -661,7 +673,7 @@ Args args_of(const Fp8Gemm& g) {
 template <bool GATED>
 int launch(const Fp8Gemm& g, cudaStream_t stream) {
   constexpr int SMEM = Room<GATED>::SMEM;
-  CUtensorMap mx, mw, my;
+  CUtensorMap mx, mw, my, mr;
   if (fp8_make_map(&mx, g.x, g.M, g.K, g.ldx, BM)) return -1;
   if (fp8_make_map(&mw, g.w, static_cast<long long>(g.groups) * g.N, g.K, g.K, GATED ? 64 : 128)) return -1;
   int sms = 0;
@@ -671,7 +683,9 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   if (fp8_allow_smem(kernel, SMEM, asked, dev)) return -1;
   Args a = args_of(g);
   memset(&my, 0, sizeof(my));
-  if (a.vec_y && fp8_make_out_map(&my, g.y, g.M, g.N, g.ldy)) return -1;
+  memset(&mr, 0, sizeof(mr));
+  if (a.vec_y && fp8_make_bf16_map(&my, g.y, g.M, g.N, g.ldy)) return -1;
+  if (a.residual && a.vec_r && fp8_make_bf16_map(&mr, g.residual, g.M, g.N, g.ldr)) return -1;
   if (g.tile_group) {
     a.tiles = reinterpret_cast<const int4*>(g.workspace);
     a.num_tiles = static_cast<const int*>(g.workspace) + 4ll * g.max_tiles;
@@ -700,7 +714,7 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, mr, a);
   if (e != cudaSuccess) {
     cudaGetLastError();  // (reported here)
     return fp8_fail(std::string("fp8 gemm launch failed: ") + cudaGetErrorString(e));
