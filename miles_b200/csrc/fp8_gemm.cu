@@ -398,10 +398,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         float amax = 0.f;
 #pragma unroll
         for (int i = 0; i < OUT; ++i) {
-          const float g = acc[i];
-          // (__expf and __fdividef are exact to a few units in the last place, where the sums before them are to about 10; where the divisor
-          // is above 2^126 the quotient is zero as it should be in fp32, less 1e-37)
-          const float a = c0 + i < half_n ? __fdividef(g, 1.f + __expf(-g)) * acc[OUT + i] : 0.f;
+          const float a = c0 + i < half_n ? f8::silu(acc[i]) * acc[OUT + i] : 0.f;
           acc[i] = a;
           amax = f8::max_nan(amax, fabsf(a));
         }

@@ -306,7 +306,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
           float a[4], amax = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            a[i] = n + i < half_n ? __fdividef(f[0][i], 1.f + __expf(-f[0][i])) * f[1][i] : 0.f;
+            a[i] = n + i < half_n ? f8::silu(f[0][i]) * f[1][i] : 0.f;
             amax = f8::max_nan(amax, fabsf(a[i]));
           }
 #pragma unroll
