@@ -22,7 +22,7 @@
 //
 // y leaves in boxes of 32 rows x 64 columns by asynchronous stores that nobody waits for until the warp's next box (their 32 KB more take a stage of
 // operands; with stores by threads, from half of that: 87 -> 73 us at 32768 x 2048 x 768, 129 -> 118 at K = 1536, 146 -> 143 at 8192 x 2048 x
-// 8192). An expert's last rows, with another's behind them in the box, and rows of y that are not 16 bytes apart are stored by threads.
+// 8192). An expert's last rows, with another's behind them in the box, and rows of y that do not begin or end at 16 bytes are stored by threads.
 //
 // Measured, us: 8192 x 24576 x 4096 gate-up 975 (1690 TFLOP/s), 8192 x 4096 x 4096 with residual 180, experts of 65536 rows, 128 of 1536 x
 // 2048 gate-up 360, 2048 x 768 226.
@@ -69,7 +69,7 @@ struct Args {
   long long ldy;
   const __nv_bfloat16* residual;
   long long ldr;
-  int vec_y, vec_r, vec_s;         // 16-byte accesses fit
+  int vec_y, vec_r, vec_s;         // 16-byte accesses fit: of y and the residual, boxes
   uint8_t* q;
   float* s;
   int* status;
@@ -658,8 +658,9 @@ Args args_of(const Fp8Gemm& g) {
   a.ldy = g.ldy;
   a.residual = static_cast<const __nv_bfloat16*>(g.residual);
   a.ldr = g.ldr;
-  a.vec_y = !g.q && g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
-  a.vec_r = g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0;
+  // (an asynchronous store ends at the 16 bytes that hold the last column, so N is a multiple of 8 elements too)
+  a.vec_y = !g.q && g.N % 8 == 0 && g.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+  a.vec_r = g.N % 8 == 0 && g.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(g.residual) & 15) == 0;
   a.vec_s = a.blocks_k % 4 == 0 && (reinterpret_cast<uintptr_t>(g.xs) & 15) == 0;
   a.q = g.q;
   a.s = g.s;

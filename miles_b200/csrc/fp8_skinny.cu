@@ -448,8 +448,8 @@ int launch(const Fp8Gemm& g, cudaStream_t stream) {
 // Few rows, or few tiles: by what either kernel costs, us. Pairs (fp8_gemm.cu) take 4.5 us and, for each round of their tiles over the SMs, 0.48 a
 // block of 128 along K and 1.2 at its end (2.5 with SwiGLU; by expert 2 more to join row tiles). The CTAs here take 5.7 and, a round, 0.61 to
 // 0.75 a block where one fits an SM; where two do, 3 and 3 a round, and 0.45 a block; or what the blocks of all of them need to arrive.
-// Measured, us, pairs / here: 24576 x 4096 gate-up, 64 rows 42 / 31, 128 rows 42 / 58; 6144 x 4096, 128 rows 21 / 16, 512 22 / 52; 4096 x 12288, 256
-// rows 50 / 36, 512 50 / 66; 128 experts, gate-up 1536 x 2048, 16 rows each 125 / 83, 64 127 / 151, 2048 x 768, 16 rows 66 / 58, 48 71 / 118.
+// Measured, us, pairs / here: 24576 x 4096 gate-up, 64 rows 40 / 30, 128 rows 41 / 56; 6144 x 4096, 128 rows 21 / 16, 512 22 / 52; 4096 x 12288, 256
+// rows 50 / 36, 512 50 / 66; 128 experts, gate-up 1536 x 2048, 16 rows each 114 / 80, 64 117 / 144, 2048 x 768, 16 rows 68 / 58, 48 69 / 119.
 bool fp8_is_skinny(const Fp8Gemm& g) {
   if (g.M <= 0) return true;
   int sms = 0;

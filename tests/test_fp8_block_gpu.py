@@ -226,6 +226,25 @@ def test_linear_into_part_of_a_wide_result(F8, T, N):
         assert (buf == 7).all()
 
 
+@pytest.mark.parametrize("T", [2945, 2970])
+@pytest.mark.parametrize("N,first,apart", [(968, 16, 16), (968, 3, 8), (1001, 8, 15), (1000, 8, 7)])
+def test_linear_of_many_rows_into_part_of_a_wide_result(F8, T, N, first, apart):
+    """The same where pairs of CTAs compute it: results and residuals whose rows are or are not multiples of 16 bytes apart, the residual as the result."""
+    g = gen(T + N)
+    x, w = F8.quantize_rows(acts(T, 144, g)), F8.quantize_weight(torch.randn(N, 144, generator=g, device=DEV).bfloat16())
+    want, err = product64(x, w)
+    buf = torch.full((T + 33, N + first + apart), 7.0, device=DEV).bfloat16()
+    out = buf[1:1 + T, first:first + N]
+    check_bf16(F8.linear(x, w, out=out), want, err)
+    for res in (acts(T, N, g), acts(T, N + 8, g)[:, 8:], acts(T, N + 3, g)[:, 2:2 + N]):
+        check_bf16(F8.linear(x, w, res, out=out), want + res.double(), err + 2.0 ** -23 * (want.abs() + res.double().abs()))
+    out.copy_(res)
+    there = F8.linear(x, w, out, out=out).clone()
+    assert torch.equal(there, F8.linear(x, w, res))
+    out.fill_(7.0)
+    assert (buf == 7).all()
+
+
 def test_linear_of_no_rows_and_bf16_rows(F8):
     w = F8.quantize_weight(torch.randn(64, 128, device=DEV).bfloat16())
     assert F8.linear(F8.quantize_rows(torch.zeros(0, 128, device=DEV).bfloat16()), w).shape == (0, 64)
