@@ -421,6 +421,11 @@ class Engine:
         if getattr(self.model, "mx_kind", None) == "fp8_block":
             self.model.refresh_block_scaled()
 
+    def serve_block_scaled(self, kind: str) -> int:
+        """Serve from block-scaled copies of the weights as they are now; returns how many there are. Called where the engine is stepped, between
+        two steps: values and scales are written one after the other, and a step in between would multiply new ones by old ones."""
+        return self.model.enable_block_scaled(kind)
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self.prefilling or self._pending is not None)
 

@@ -55,9 +55,8 @@ def register_extra(app, engine, state: dict) -> None:
         holds now; called by the trainer after a weight update when ``--weight-sync-quant`` is set."""
         b = await req.json()
         fmt = b.get("format", "none")
-        fn = getattr(engine.model, "enable_block_scaled", None)
-        if fmt in ("mxfp8", "nvfp4", "fp8_block") and fn is not None:
-            return {"success": True, "num_tensors": await asyncio.to_thread(fn, fmt)}
+        if fmt in ("mxfp8", "nvfp4", "fp8_block") and hasattr(engine.model, "enable_block_scaled"):
+            return {"success": True, "num_tensors": engine.serve_block_scaled(fmt)}  # (on the event loop, which steps the engine)
         return {"success": False, "reason": f"format {fmt!r} is not served by this engine"}
 
     @app.get("/parallelism_config")

@@ -211,7 +211,7 @@ class B200Qwen3:
         from ..ops.fp8_block import quantize_weight
 
         old = self.mx if getattr(self, "mx_kind", None) == "fp8_block" else {}
-        self.mx_kind, self.mx = "fp8_block", {}
+        copies = {}  # takes the place of the old ones as a whole: whoever computes meanwhile finds those
         for name, w in self.store.params.items():
             halves = 2 if name.endswith(("mlp.gate_up.weight", "moe.w1")) else 1
             # (rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a gate-up product leaves)
@@ -223,8 +223,9 @@ class B200Qwen3:
                 kept.q.view(torch.uint8).copy_(q.q.view(torch.uint8))
                 kept.scales.copy_(q.scales)
                 q = kept
-            self.mx[w.data_ptr()] = q
-        return len(self.mx)
+            copies[w.data_ptr()] = q
+        self.mx_kind, self.mx = "fp8_block", copies
+        return len(copies)
 
     def _fp8(self, w, rows: int):
         """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None: up to ``SMALL_T`` rows the fused kernels on bf16 weights take fewer
@@ -232,12 +233,14 @@ class B200Qwen3:
         mx = getattr(self, "mx", None)
         return mx.get(w.data_ptr()) if mx and self.mx_kind == "fp8_block" and rows > self.SMALL_T else None
 
-    def _fp8_layer(self, i: int, rows: int) -> bool:
-        """Whether layer i's activations pass from product to product in 8 bits: not where they are exchanged with other ranks or normed once more."""
+    def _fp8_layer(self, i: int, rows: int) -> Optional[tuple]:
+        """The 8-bit copies of layer i (q, k and v, output, and both products behind the norm) if its activations pass from product to product in
+        8 bits: not where they are exchanged with other ranks or normed once more. They are looked up once, so that a layer is computed from one set of copies."""
         if self.tp is not None or self.ep is not None or self.cfg.post_norms or not getattr(self, "mx", None):
-            return False
+            return None
         names = ("moe.w1", "moe.w2") if self.cfg.layer_is_moe(i) else ("mlp.gate_up.weight", "mlp.down.weight")
-        return all(self._fp8(self.store.params[f"layers.{i}.{n}"], rows) is not None for n in ("attn.qkv.weight", "attn.o.weight", *names))
+        copies = tuple(self._fp8(self.store.params[f"layers.{i}.{n}"], rows) for n in ("attn.qkv.weight", "attn.o.weight", *names))
+        return copies if all(c is not None for c in copies) else None
 
     def use_block_scaled(self, kind: str, operands: dict) -> None:
         """Serve from block-scaled copies that something else keeps up to date (``{parameter name: MxOperand}``, e.g.
@@ -352,8 +355,9 @@ class B200Qwen3:
         mx = getattr(self, "mx", None)
         if mx and self.mx_kind == "fp8_block":
             tokens = plan.ids.shape[0]
-            if not keep and scatter is None and self._fp8(w1, tokens) is not None and self._fp8(w2, tokens) is not None:
-                return None, None, self._fp8_experts(xp, plan, w1, w2)
+            copies = self._fp8(w1, tokens), self._fp8(w2, tokens)
+            if not keep and scatter is None and copies[0] is not None and copies[1] is not None:
+                return None, None, self._fp8_experts(xp, plan, *copies)
         elif mx and not keep and scatter is None and w1.data_ptr() in mx and w2.data_ptr() in mx and plan.align == 128:
             # rows of xp past the live tiles are never written: the per-tensor scale of NVFP4 must not look at them
             gu = self._mx_linear(xp, mx[w1.data_ptr()], plan.tile_group, plan.num_tiles, I2, getattr(plan, "amax_in", None))
@@ -379,20 +383,20 @@ class B200Qwen3:
         self.launches += 2
         return (gu, act, yp) if keep else (None, None, yp)
 
-    def _fp8_experts(self, xp, plan: MoeCtx, w1, w2):
+    def _fp8_experts(self, xp, plan: MoeCtx, w1_8, w2_8):
         """Both products of rows in expert order (bf16, or 8-bit rows) from the experts' 8-bit copies."""
         from ..ops import fp8_block as F8
 
         if not isinstance(xp, F8.Fp8Rows):
             xp = F8.quantize_rows(xp)  # (rows past the live ones hold anything, and are not read)
             self.launches += 1
-        act = F8.grouped_gated_linear(xp, self.mx[w1.data_ptr()], plan.tile_group, plan.num_tiles, self.status)
-        yp = F8.grouped_linear(act, self.mx[w2.data_ptr()], plan.tile_group, plan.num_tiles, status=self.status)
-        self.launches += 2 * self.C.fp8_grouped_launches(plan.max_rows, w1.shape[0])
+        act = F8.grouped_gated_linear(xp, w1_8, plan.tile_group, plan.num_tiles, self.status)
+        yp = F8.grouped_linear(act, w2_8, plan.tile_group, plan.num_tiles, status=self.status)
+        self.launches += 2 * self.C.fp8_grouped_launches(plan.max_rows, w1_8.q.shape[0])
         return yp
 
-    def moe_forward(self, i, h2, replay_ids=None, record=None, keep=False, residual=None, serving=False, rows=None):
-        """``rows``: ``h2`` as 8-bit rows, for experts that are served from 8-bit copies."""
+    def moe_forward(self, i, h2, replay_ids=None, record=None, keep=False, residual=None, serving=False, fp8=None):
+        """``fp8``: ``h2`` as 8-bit rows and the 8-bit copies of both expert weights, for a layer that is served from them."""
         cfg, P, C = self.cfg, self.store.params, self.C
         p = f"layers.{i}.moe."
         ids, w, probs = self._route(h2, P[p + "router.weight"], replay_ids, P.get(p + "router.bias"), serving)
@@ -413,11 +417,12 @@ class B200Qwen3:
         use_mx = bool(getattr(self, "mx", None)) and self.mx_kind != "fp8_block" and not keep and h2.shape[0] > 32
         plan = self._permute_plan(ids, cfg.num_experts, 64 if keep else (128 if use_mx else 1))
         plan.w, plan.probs = w, probs
-        if rows is not None:
+        if fp8 is not None:
             from ..ops.fp8_block import permute_rows
 
+            rows, w1_8, w2_8 = fp8
             gu = act = xp = None
-            yp = self._fp8_experts(permute_rows(rows, plan.src, plan.num_tiles, cfg.moe_top_k), plan, P[p + "w1"], P[p + "w2"])
+            yp = self._fp8_experts(permute_rows(rows, plan.src, plan.num_tiles, cfg.moe_top_k), plan, w1_8, w2_8)
         else:
             xp = C.moe_permute(h2, plan.src, plan.num_tiles, cfg.moe_top_k)
             if use_mx and self.mx_kind == "nvfp4":
@@ -511,14 +516,15 @@ class B200Qwen3:
         return dh2
 
     # ------------------------------------------------------------------ layer forward / backward
-    def _attn_qkv(self, i, x, positions, meta: Optional[InferMeta], kv_cache, fp8: bool = False):
+    def _attn_qkv(self, i, x, positions, meta: Optional[InferMeta], kv_cache, qkv8=None):
+        """``qkv8``: the 8-bit copy of the weight, for a layer that is served from such copies."""
         cfg, P, C = self.cfg, self.store.params, self.C
         p = f"layers.{i}."
-        if fp8:
+        if qkv8 is not None:
             from ..ops.fp8_block import rmsnorm_rows
 
             h1, rstd1 = rmsnorm_rows(x, P[p + "ln1.weight"], cfg.rms_eps)[0], None
-            qkv = self._fp8_linear(h1, self.mx[P[p + "attn.qkv.weight"].data_ptr()])
+            qkv = self._fp8_linear(h1, qkv8)
         else:
             h1, rstd1 = C.rmsnorm_fwd(x, None, P[p + "ln1.weight"], cfg.rms_eps)
             qkv = self.linear(h1, P[p + "attn.qkv.weight"], serving=meta is not None)
@@ -578,7 +584,7 @@ class B200Qwen3:
             return y
         serving = meta is not None
         fp8 = self._fp8_layer(i, x.shape[0])
-        h1, rstd1, qkv, q, k, _, _ = self._attn_qkv(i, x, positions, meta, kv_cache, fp8)
+        h1, rstd1, qkv, q, k, _, _ = self._attn_qkv(i, x, positions, meta, kv_cache, fp8 and fp8[0])
         scale = cfg.head_dim ** -0.5
         if meta is not None and not meta.is_prefill:
             att = torch.empty_like(q)
@@ -600,7 +606,7 @@ class B200Qwen3:
         else:
             att, _ = self.attention(q, k, self._v_view(qkv), cu)
         if fp8:
-            return self._mlp_fp8(i, att.view(att.shape[0], -1), x, replay_ids, record, serving)
+            return self._mlp_fp8(i, att.view(att.shape[0], -1), x, replay_ids, record, serving, *fp8[1:])
         h2, _, x2 = self._o_proj_ln2(i, att.view(att.shape[0], -1), x, serving)
         if cfg.layer_is_moe(i):
             if (meta is not None and not meta.is_prefill and replay_ids is None and getattr(self.ep, "low_latency", False)
@@ -616,21 +622,21 @@ class B200Qwen3:
             return yn.add_(x2)
         return self._row_parallel(act, P[p + "mlp.down.weight"], x2, serving)
 
-    def _mlp_fp8(self, i, att2, x, replay_ids, record, serving):
+    def _mlp_fp8(self, i, att2, x, replay_ids, record, serving, o8, first8, second8):
         """What follows attention, from the weights' 8-bit copies: every product's input leaves the kernel before it in 8 bits."""
         from ..ops.fp8_block import gated_linear, rmsnorm_rows
 
         cfg, P = self.cfg, self.store.params
         p = f"layers.{i}."
         moe = cfg.layer_is_moe(i)
-        o = self._fp8_linear(att2, self.mx[P[p + "attn.o.weight"].data_ptr()])
+        o = self._fp8_linear(att2, o8)
         rows, x2, h2 = rmsnorm_rows(o, P[p + "ln2.weight"], cfg.rms_eps, x, keep=moe)  # (the router reads bf16)
         self.launches += 1
         if moe:
-            return self.moe_forward(i, h2, replay_ids, record, keep=False, residual=x2, serving=serving, rows=rows)[0]
-        act = gated_linear(rows, self.mx[P[p + "mlp.gate_up.weight"].data_ptr()], self.status)
+            return self.moe_forward(i, h2, replay_ids, record, keep=False, residual=x2, serving=serving, fp8=(rows, first8, second8))[0]
+        act = gated_linear(rows, first8, self.status)
         self.launches += 1
-        return self._fp8_linear(act, self.mx[P[p + "mlp.down.weight"].data_ptr()], x2)
+        return self._fp8_linear(act, second8, x2)
 
     def _full_kv(self, prefix, k, v, kc, vc):
         """``PrefixInfo.full_kv`` in one launch for caches of the activations' type."""
