@@ -185,6 +185,7 @@ class Engine:
         self._rid = itertools.count()
         self.use_cuda_graph = self.on_gpu if use_cuda_graph is None else use_cuda_graph
         self._graphs: dict = {}
+        self._graphs_of = 0  # (if there are any) the model's `mx_generation` that they were captured with
         self._alloc_decode_buffers()
         self.stats = {"prefill_tokens": 0, "decode_tokens": 0, "decode_steps": 0, "retracted": 0}
         # host wall time and count of decode iterations per row bucket (the GPU is the bottleneck of a decode
@@ -930,7 +931,7 @@ class Engine:
             self._append_token(r, int(tok_l[i]), float(lp_l[i]))
 
     def _can_look_ahead(self, pend: dict) -> bool:
-        if not self.overlap_decode or self.sync is not None or self.paused or self.waiting:
+        if not self.overlap_decode or self.sync is not None or self.paused or self.waiting or not self._graphs_current():
             return False
         reqs = pend["reqs"]
         if len(reqs) != len(self.running) or any(a is not b for a, b in zip(reqs, self.running)):
@@ -945,7 +946,7 @@ class Engine:
     def _can_launch_ahead(self, pend: dict, bucket: int) -> bool:
         """Lockstep engines: may the next step be launched before the host has seen the step in flight? Only when
         nothing about the batch can change: same requests, same row bound, nobody certain to stop, pages at hand."""
-        if not self.overlap_decode or self.paused or self.waiting or bucket != self._rows_B:
+        if not self.overlap_decode or self.paused or self.waiting or bucket != self._rows_B or not self._graphs_current():
             return False
         reqs = pend["reqs"]
         if len(reqs) != len(self.running) or any(a is not b for a, b in zip(reqs, self.running)):
@@ -1040,9 +1041,15 @@ class Engine:
         self.d_step[:B] += act
         return torch.stack(record, 1) if want_routes else None
 
+    def _graphs_current(self) -> bool:
+        """Whether captured steps read the weights' copies that the model serves from now."""
+        return not self._graphs or self._graphs_of == getattr(self.model, "mx_generation", 0)
+
     def _run_decode(self, B: int, want_routes: bool):
         if not (self.use_cuda_graph and self.on_gpu):
             return self._decode_body(B, want_routes)
+        if not self._graphs_current():  # (never a step ahead: capturing starts from what the host has seen)
+            self._graphs.clear()
         key = (B, want_routes)
         entry = self._graphs.get(key)
         if entry is None:
@@ -1060,6 +1067,7 @@ class Engine:
                 out = self._decode_body(B, want_routes)
             entry = (g, out, per_replay, self.d_logits)
             self._graphs[key] = entry
+            self._graphs_of = getattr(self.model, "mx_generation", 0)
             if hasattr(self.model, "launches"):
                 self.model.launches -= 2 * per_replay  # neither the warm-up nor the capture pass produced tokens
             # the warm-up run advanced the device-side decode state; rewind it before the first real replay

@@ -97,6 +97,18 @@ def _out_of_memory(e: RuntimeError) -> bool:
     return isinstance(e, torch.OutOfMemoryError) or "out of memory" in str(e)
 
 
+def _written_over(old, new) -> bool:
+    """Whether ``old`` (a weight's block-scaled copy) could take the values of ``new`` where it is; it has them then."""
+    a, b = vars(old), vars(new)
+    if type(old) is not type(new) or any(torch.is_tensor(v) != torch.is_tensor(a[k]) or (v.shape != a[k].shape if torch.is_tensor(v) else v != a[k])
+                                         for k, v in b.items()):
+        return False
+    for k, v in b.items():
+        if torch.is_tensor(v):
+            a[k].view(torch.uint8).copy_(v.view(torch.uint8))
+    return True
+
+
 class B200Qwen3:
     def __init__(self, cfg: ModelConfig, store: ParamStore, ep=None, tp=None):
         assert cfg.head_dim == 128, "the sm_100a attention/rope kernels are specialised for head_dim 128"
@@ -109,6 +121,7 @@ class B200Qwen3:
         self.dev = store.device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.dev)
         self.launches = 0  # number of this library's kernels launched (reported by the benchmark)
+        self.mx_generation = 0  # changes with the addresses of the block-scaled copies that are served from (enable_block_scaled)
         self._decode_scratch: Optional[torch.Tensor] = None
         self._tiles = TileCache()
         self.cp_ctx = None  # (sample lengths, cp size, cp rank, group, comm, layout) while a context-parallel micro-batch runs
@@ -190,42 +203,46 @@ class B200Qwen3:
         """Serve the projections and experts from MXFP8 / NVFP4 copies of the weights (`csrc/gemm_mx.cu`) whenever
         more than 32 rows are multiplied, or from E4M3 copies with a scale for each 128 x 128 (``fp8_block``, `ops/fp8_block.py`) whenever more
         than ``SMALL_T`` are; the few-row decode kernels keep streaming the bf16 weights. Meant for a
-        model object that only the rollout engine uses. Call again (or `refresh_block_scaled`) after a weight update.
+        model object that only the rollout engine uses. Call again (or `refresh_block_scaled`) after a weight update: copies
+        of the same format are written where they are, since captured decode steps read them there.
         Returns the number of tensors quantised."""
-        if kind == "fp8_block":
-            return self._enable_fp8_block()
+        if kind not in ("mxfp8", "nvfp4", "fp8_block"):
+            raise ValueError(f"unknown block-scaled kind {kind!r}")
+        quantize = self._quantize_fp8_block if kind == "fp8_block" else self._quantize_mx
+        if getattr(self, "mx_kind", None) != kind or getattr(self, "mx_external", False):
+            # steps captured until now read other copies or none, and must be gone before what they read is
+            self.mx_generation, self.mx_external = self.mx_generation + 1, False
+            self.mx_kind, self.mx = kind, {}
+        copies, placed = {}, False  # takes the place of the old ones as a whole: whoever computes meanwhile finds those
+        for name, w in self.store.params.items():
+            q = quantize(name, w, kind) if name.endswith(self.MX_SUFFIXES) else None
+            if q is None:
+                continue
+            old = self.mx.get(w.data_ptr())
+            if old is not None and _written_over(old, q):
+                q = old
+            else:
+                placed = True
+            copies[w.data_ptr()] = q
+        self.mx_generation += placed or copies.keys() != self.mx.keys()
+        self.mx = copies
+        return len(copies)
+
+    @staticmethod
+    def _quantize_mx(name, w, kind):
         from ..ops.mx_gemm import quantize_operand
 
         step = 128 if kind == "mxfp8" else 256
-        self.mx_kind, self.mx = kind, {}
-        for name, w in self.store.params.items():
-            if not name.endswith(self.MX_SUFFIXES):
-                continue
-            w2 = w.reshape(-1, w.shape[-1])
-            if w2.shape[1] % step or w2.shape[0] % 128:
-                continue
-            self.mx[w.data_ptr()] = quantize_operand(w2, kind)
-        return len(self.mx)
+        w2 = w.reshape(-1, w.shape[-1])
+        return None if w2.shape[1] % step or w2.shape[0] % 128 else quantize_operand(w2, kind)
 
-    def _enable_fp8_block(self) -> int:
+    @staticmethod
+    def _quantize_fp8_block(name, w, kind):
         from ..ops.fp8_block import quantize_weight
 
-        old = self.mx if getattr(self, "mx_kind", None) == "fp8_block" else {}
-        copies = {}  # takes the place of the old ones as a whole: whoever computes meanwhile finds those
-        for name, w in self.store.params.items():
-            halves = 2 if name.endswith(("mlp.gate_up.weight", "moe.w1")) else 1
-            # (rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a gate-up product leaves)
-            if not name.endswith(self.MX_SUFFIXES) or w.shape[-1] % 16 or w.shape[-2] % (16 * halves):
-                continue
-            q = quantize_weight(w, halves)
-            kept = old.get(w.data_ptr())
-            if kept is not None and kept.q.shape == q.q.shape:  # captured decode steps read the copies where they were
-                kept.q.view(torch.uint8).copy_(q.q.view(torch.uint8))
-                kept.scales.copy_(q.scales)
-                q = kept
-            copies[w.data_ptr()] = q
-        self.mx_kind, self.mx = "fp8_block", copies
-        return len(copies)
+        halves = 2 if name.endswith(("mlp.gate_up.weight", "moe.w1")) else 1
+        # (rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a gate-up product leaves)
+        return None if w.shape[-1] % 16 or w.shape[-2] % (16 * halves) else quantize_weight(w, halves)
 
     def _fp8(self, w, rows: int):
         """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None: up to ``SMALL_T`` rows the fused kernels on bf16 weights take fewer
@@ -245,6 +262,7 @@ class B200Qwen3:
     def use_block_scaled(self, kind: str, operands: dict) -> None:
         """Serve from block-scaled copies that something else keeps up to date (``{parameter name: MxOperand}``, e.g.
         the buffers a peer-memory weight push quantises into)."""
+        self.mx_generation += 1
         self.mx_kind, self.mx_external = kind, True
         self.mx = {self.store.params[n].data_ptr(): op for n, op in operands.items() if n in self.store.params}
 
