@@ -39,6 +39,7 @@ class MoeCtx:
     max_rows: int
     align: int = 1
     pairs: int = 0  # routed pairs to expect among max_rows (0: as many)
+    tokens: int = 0  # of the pass, where all experts are this rank's own (0: the rows come from other ranks, too)
 
     def gated(self) -> bool:
         """Whether the gate-up product of these rows takes SwiGLU into its epilogue (csrc/gemm.cu). Experts of few rows stream their weights, which
@@ -203,7 +204,7 @@ class B200Qwen3:
         """Serve the projections and experts from MXFP8 / NVFP4 copies of the weights (`csrc/gemm_mx.cu`) whenever
         more than 32 rows are multiplied, or from E4M3 copies with a scale for each 128 x 128 (``fp8_block``, `ops/fp8_block.py`) whenever more
         than ``SMALL_T`` are; the few-row decode kernels keep streaming the bf16 weights. Meant for a
-        model object that only the rollout engine uses. Call again (or `refresh_block_scaled`) after a weight update: copies
+        model object that only the rollout engine uses. Experts of an expert-parallel model stay in bf16. Call again (or `refresh_block_scaled`) after a weight update: copies
         of the same format are written where they are, since captured decode steps read them there.
         Returns the number of tensors quantised."""
         if kind not in ("mxfp8", "nvfp4", "fp8_block"):
@@ -214,8 +215,10 @@ class B200Qwen3:
             self.mx_generation, self.mx_external = self.mx_generation + 1, False
             self.mx_kind, self.mx = kind, {}
         copies, placed = {}, False  # takes the place of the old ones as a whole: whoever computes meanwhile finds those
+        # (experts that other ranks' rows reach are multiplied in bf16: the exchanges' plans have no rows to spare for whole tiles, and no count of tokens)
+        served = self.MX_SUFFIXES if self.ep is None else tuple(n for n in self.MX_SUFFIXES if not n.startswith("moe."))
         for name, w in self.store.params.items():
-            q = quantize(name, w, kind) if name.endswith(self.MX_SUFFIXES) else None
+            q = quantize(name, w, kind) if name.endswith(served) else None
             if q is None:
                 continue
             old = self.mx.get(w.data_ptr())
@@ -372,8 +375,7 @@ class B200Qwen3:
         I2 = w1.shape[1]
         mx = getattr(self, "mx", None)
         if mx and self.mx_kind == "fp8_block":
-            tokens = plan.ids.shape[0]
-            copies = self._fp8(w1, tokens), self._fp8(w2, tokens)
+            copies = self._fp8(w1, plan.tokens), self._fp8(w2, plan.tokens)
             if not keep and scatter is None and copies[0] is not None and copies[1] is not None:
                 return None, None, self._fp8_experts(xp, plan, *copies)
         elif mx and not keep and scatter is None and w1.data_ptr() in mx and w2.data_ptr() in mx and plan.align == 128:
@@ -434,7 +436,7 @@ class B200Qwen3:
             return self.ep.moe_forward(self, i, h2, ids, w, probs, keep, residual)
         use_mx = bool(getattr(self, "mx", None)) and self.mx_kind != "fp8_block" and not keep and h2.shape[0] > 32
         plan = self._permute_plan(ids, cfg.num_experts, 64 if keep else (128 if use_mx else 1))
-        plan.w, plan.probs = w, probs
+        plan.w, plan.probs, plan.tokens = w, probs, h2.shape[0]
         if fp8 is not None:
             from ..ops.fp8_block import permute_rows
 
