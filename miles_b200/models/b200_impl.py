@@ -239,13 +239,23 @@ class B200Qwen3:
         w2 = w.reshape(-1, w.shape[-1])
         return None if w2.shape[1] % step or w2.shape[0] % 128 else quantize_operand(w2, kind)
 
-    @staticmethod
-    def _quantize_fp8_block(name, w, kind):
+    def _quantize_fp8_block(self, name, w, kind):
         from ..ops.fp8_block import quantize_weight
 
-        halves = 2 if name.endswith(("mlp.gate_up.weight", "moe.w1")) else 1
-        # (rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a gate-up product leaves)
-        return None if w.shape[-1] % 16 or w.shape[-2] % (16 * halves) else quantize_weight(w, halves)
+        # gate and up rows get blocks of their own where a gated product reads them, and those of one matrix where `linear` does
+        halves = 2 if name.endswith("moe.w1") or (name.endswith("mlp.gate_up.weight") and self._fp8_chains(int(name.split(".")[1]))) else 1
+        return quantize_weight(w, halves) if self._fp8_fits(w, halves) else None
+
+    @staticmethod
+    def _fp8_fits(w, halves: int = 1) -> bool:
+        """Rows of 8-bit values are a multiple of 16 wide: those of the input, and those that a product leaves."""
+        return w.shape[-1] % 16 == 0 and w.shape[-2] % (16 * halves) == 0
+
+    def _fp8_chains(self, i: int) -> bool:
+        """Whether the activations of a dense layer i can pass from product to product in 8 bits."""
+        P = self.store.params
+        return (self.tp is None and self.ep is None and not self.cfg.post_norms and self._fp8_fits(P[f"layers.{i}.mlp.gate_up.weight"], 2)
+                and all(self._fp8_fits(P[f"layers.{i}.{n}"]) for n in ("attn.qkv.weight", "attn.o.weight", "mlp.down.weight")))
 
     def _fp8(self, w, rows: int):
         """The 8-bit copy that a product of ``rows`` rows with ``w`` reads, or None: up to ``SMALL_T`` rows the fused kernels on bf16 weights take fewer
@@ -297,7 +307,7 @@ class B200Qwen3:
         mx = getattr(self, "mx", None)
         if mx and out_dtype == torch.bfloat16 and self.mx_kind == "fp8_block":
             w8 = self._fp8(w, T)
-            if w8 is not None:
+            if w8 is not None and w8.whole:
                 return self._fp8_linear(x, w8)
         elif mx and T > 32 and out_dtype == torch.bfloat16 and w.data_ptr() in mx:
             return self._mx_linear(x.contiguous(), mx[w.data_ptr()])
@@ -316,8 +326,8 @@ class B200Qwen3:
         """``(gate | up if kept, silu(gate) * up)`` for a gate-up weight [2I, K]: one launch where tiles of 128 such columns fill
         the device (csrc/gemm.cu), else the product and the activation. The same bits either way."""
         T, I = x.shape[0], w.shape[0] // 2
-        mx = getattr(self, "mx", None)
-        if T > 128 and I % 8 == 0 and -(-T // 128) * -(-I // 128) >= 148 and x.is_contiguous() and not (mx and w.data_ptr() in mx):
+        copy = (getattr(self, "mx", None) or {}).get(w.data_ptr())
+        if T > 128 and I % 8 == 0 and -(-T // 128) * -(-I // 128) >= 148 and x.is_contiguous() and (copy is None or not getattr(copy, "whole", True)):
             gu = torch.empty(T, 2 * I, dtype=torch.bfloat16, device=x.device) if keep else None
             act = torch.empty(T, I, dtype=torch.bfloat16, device=x.device)
             self.C.gated_gemm(x, w, act, gu, None, None, self.status)

@@ -46,6 +46,11 @@ class Fp8Weight:
     scales: torch.Tensor   # fp32 [halves * ceil(N / halves / 128), ceil(K / 128)], or [experts, ...]
     halves: int = 1        # 2: a gate-up weight whose halves have blocks of their own (they do anyway if they are multiples of 128)
 
+    @property
+    def whole(self) -> bool:
+        """Whether its blocks are also those of one matrix of all its rows, so that the ungated products read it."""
+        return self.halves == 1 or self.q.shape[-2] // 2 % BLOCK == 0
+
     def dequantize(self) -> torch.Tensor:
         def split(t):
             return t.unflatten(-2, (self.halves, t.shape[-2] // self.halves))
