@@ -12,6 +12,7 @@ continue, cache flush and memory release / resume.
 """
 from __future__ import annotations
 
+import contextlib
 import itertools
 import time
 import zlib
@@ -182,6 +183,7 @@ class Engine:
         self.fed: dict = {}         # sequences whose tokens are given by the caller (feed), by id
         self.paused = False
         self.weight_version = 0
+        self._copies_stale = False  # weights have changed since the model's 8-bit copies of them were made
         self._rid = itertools.count()
         self.use_cuda_graph = self.on_gpu if use_cuda_graph is None else use_cuda_graph
         self._graphs: dict = {}
@@ -204,8 +206,6 @@ class Engine:
             # prefill or decode step before any position of it is read.
             self.kv_cache = self.layout.allocate(slots, sequences, self.dev, self.kv_storage)
             return
-        import contextlib
-
         with (self._saver.region(self._kv_tag) if self._saver is not None else contextlib.nullcontext()):
             self.kv_cache = self.layout.allocate(slots, sequences, self.dev)
 
@@ -417,15 +417,31 @@ class Engine:
         self.weight_version = self.weight_version + 1 if version is None else int(version)
         return self.weight_version
 
+    @contextlib.contextmanager
+    def weights_change(self):
+        """Around whatever writes to the weights: 8-bit copies of them are quantised anew before anything else is computed, also if the writing
+        ends halfway. `weights_arrived` does so at once."""
+        try:
+            yield
+        finally:
+            self._copies_stale = True
+
     def weights_arrived(self) -> None:
         """Weights changed in place: an engine that serves from 8-bit copies (``fp8_block``) quantises them anew, where captured steps read them."""
         if getattr(self.model, "mx_kind", None) == "fp8_block":
             self.model.refresh_block_scaled()
+        self._copies_stale = False
+
+    def _current_copies(self) -> None:
+        if self._copies_stale:
+            self.weights_arrived()
 
     def serve_block_scaled(self, kind: str) -> int:
         """Serve from block-scaled copies of the weights as they are now; returns how many there are. Called where the engine is stepped, between
         two steps: values and scales are written one after the other, and a step in between would multiply new ones by old ones."""
-        return self.model.enable_block_scaled(kind)
+        n = self.model.enable_block_scaled(kind)
+        self._copies_stale = False
+        return n
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self.prefilling or self._pending is not None)
@@ -510,6 +526,8 @@ class Engine:
         if self.kv_cache is None or self._kv_paused:
             return []
         before = set(self.finished)
+        if not self.paused:
+            self._current_copies()
         admitted = [] if self.paused else self._admit()
         local = 2 if admitted else (1 if ((self.running and not self.paused) or self._pending is not None) else 0)
         bucket = None
@@ -1087,6 +1105,7 @@ class Engine:
         every entry (``[wanted, vocab]`` fp32). Sequences fed this way share pages and state rows with generation;
         :meth:`end_feed` gives them back."""
         self._drain_pending()
+        self._current_copies()
         ps = self.page_size
         out: list = [None] * len(entries)
         portions, singles = [], []
@@ -1152,6 +1171,7 @@ class Engine:
         n = len(ids)
         if n < 2:
             return {"logprobs": [None] * n, "top": [None] * n}
+        self._current_copies()
         dev = self.dev
         tok = torch.tensor(ids, dtype=torch.int32, device=dev)
         pos = torch.arange(n, dtype=torch.int32, device=dev)

@@ -86,10 +86,11 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
         n = 0
         from ..models.hf_mapping import param_or_hf_view
 
-        for name, tensor in take_bucket(body["bucket_id"]):
-            dst = param_or_hf_view(engine.cfg, engine.store, name)  # native or HuggingFace tensor name
-            dst.copy_(tensor.to(dst.dtype))
-            n += 1
+        with engine.weights_change():
+            for name, tensor in take_bucket(body["bucket_id"]):
+                dst = param_or_hf_view(engine.cfg, engine.store, name)  # native or HuggingFace tensor name
+                dst.copy_(tensor.to(dst.dtype))
+                n += 1
         if body.get("weight_version") is not None:
             engine.weights_arrived()
             engine.update_weight_version(body["weight_version"])
@@ -100,7 +101,8 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
         body = await req.json()
         from ..checkpoint import load_hf
 
-        n = load_hf(engine.cfg, engine.store, body["model_path"], strict=False)
+        with engine.weights_change():
+            n = load_hf(engine.cfg, engine.store, body["model_path"], strict=False)
         engine.weights_arrived()
         if body.get("weight_version") is not None:
             engine.update_weight_version(body["weight_version"])
@@ -150,8 +152,10 @@ def build_app(engine: Engine, tokenizer=None, model_path: str = ""):
             snapshot["flat"] = {g: t.clone() for g, t in engine.store.flat.items()}
             return {"success": True}
         if action == "reset_tensors":
-            for t in engine.store.flat.values():
-                t.zero_()
+            with engine.weights_change():
+                for t in engine.store.flat.values():
+                    t.zero_()
+            engine.weights_arrived()
             return {"success": True}
         if action == "compare":
             ok = all((engine.store.flat[g] == t).all().item() for g, t in snapshot.get("flat", {}).items())

@@ -31,7 +31,8 @@ def register_extra(app, engine, state: dict) -> None:
         b = await req.json()
         from ..weight_sync.broadcast import receive_bucket
 
-        n = await asyncio.to_thread(receive_bucket, b, engine.store)
+        with engine.weights_change():
+            n = await asyncio.to_thread(receive_bucket, b, engine.store)
         if b.get("weight_version") is not None:
             engine.weights_arrived()
             engine.update_weight_version(b["weight_version"])
@@ -43,7 +44,8 @@ def register_extra(app, engine, state: dict) -> None:
         b = await req.json()
         from ..weight_sync.disk_delta import apply_delta_dir
 
-        n = await asyncio.to_thread(apply_delta_dir, engine.store, b["path"])
+        with engine.weights_change():
+            n = await asyncio.to_thread(apply_delta_dir, engine.store, b["path"])
         engine.weights_arrived()
         if b.get("weight_version") is not None:
             engine.update_weight_version(b["weight_version"])
@@ -79,7 +81,8 @@ def register_extra(app, engine, state: dict) -> None:
             raise HTTPException(409, f"adapter {name!r} is already loaded")
         tensors = dict(take_bucket(b["bucket_id"]))
         scale = float(b.get("scaling", 1.0))
-        merge_adapter_into(engine.store, tensors, scale)
+        with engine.weights_change():
+            merge_adapter_into(engine.store, tensors, scale)
         engine.weights_arrived()
         state["adapters"][name] = (tensors, scale)
         return {"success": True, "loaded_adapters": sorted(state["adapters"])}
@@ -92,7 +95,8 @@ def register_extra(app, engine, state: dict) -> None:
         ad = state.setdefault("adapters", {}).pop(b["lora_name"], None)
         if ad is None:
             raise HTTPException(404, f"adapter {b['lora_name']!r} is not loaded")
-        merge_adapter_into(engine.store, ad[0], -ad[1])
+        with engine.weights_change():
+            merge_adapter_into(engine.store, ad[0], -ad[1])
         engine.weights_arrived()
         return {"success": True, "loaded_adapters": sorted(state["adapters"])}
 
