@@ -183,7 +183,8 @@ class Engine:
         self.fed: dict = {}         # sequences whose tokens are given by the caller (feed), by id
         self.paused = False
         self.weight_version = 0
-        self._copies_stale = False  # weights have changed since the model's 8-bit copies of them were made
+        self._copies_stale = False                # weights have changed since the model's 8-bit copies of them were made
+        self._copies_of: Optional[tuple] = None   # the writes to the weights that copies made by `weights_arrived` have seen
         self._rid = itertools.count()
         self.use_cuda_graph = self.on_gpu if use_cuda_graph is None else use_cuda_graph
         self._graphs: dict = {}
@@ -430,7 +431,12 @@ class Engine:
         """Weights changed in place: an engine that serves from 8-bit copies (``fp8_block``) quantises them anew, where captured steps read them."""
         if getattr(self.model, "mx_kind", None) == "fp8_block":
             self.model.refresh_block_scaled()
+            self._copies_of = self._weight_writes()
         self._copies_stale = False
+
+    def _weight_writes(self) -> tuple:
+        """Counts the writes to the weights, as PyTorch does."""
+        return tuple(t._version for t in self.store.flat.values())
 
     def _current_copies(self) -> None:
         if self._copies_stale:
@@ -438,9 +444,13 @@ class Engine:
 
     def serve_block_scaled(self, kind: str) -> int:
         """Serve from block-scaled copies of the weights as they are now; returns how many there are. Called where the engine is stepped, between
-        two steps: values and scales are written one after the other, and a step in between would multiply new ones by old ones."""
-        n = self.model.enable_block_scaled(kind)
-        self._copies_stale = False
+        two steps: values and scales are written one after the other, and a step in between would multiply new ones by old ones. Copies that
+        `weights_arrived` has made of these very weights are not made twice."""
+        model = self.model
+        if kind == getattr(model, "mx_kind", None) == "fp8_block" and not self._copies_stale and self._copies_of == self._weight_writes():
+            return len(model.mx)
+        n = model.enable_block_scaled(kind)
+        self._copies_stale, self._copies_of = False, None
         return n
 
     def has_work(self) -> bool:

@@ -1,4 +1,4 @@
-"""No answer comes from 8-bit copies of weights that have changed since, whichever endpoint changed them."""
+"""No answer comes from 8-bit copies of weights that have changed since, whichever endpoint changed them; and one update quantises them once."""
 import pytest
 import torch
 
@@ -104,3 +104,17 @@ def test_a_paused_engine_waits_for_the_last_bucket(s):
     s.c.post("/update_weight_version", json={"new_version": 2})
     s.c.post("/continue_generation")
     assert generate(s).status_code == 200 and s.seen == [0.5]
+
+
+def test_one_update_quantises_once(s):
+    s.c.post("/update_weights_from_tensor", json={"bucket_id": s.bucket(0.5)})
+    s.c.post("/update_weight_version", json={"new_version": 2})
+    assert s.c.post("/requantize_weights", json={"format": "fp8_block"}).json() == {"success": True, "num_tensors": 2}
+    assert s.seen == [0.5] and s.made == []
+    s.fill(0.75)  # (a write that no endpoint made)
+    assert s.c.post("/requantize_weights", json={"format": "fp8_block"}).json()["num_tensors"] == 7
+    s.c.post("/update_weights_from_tensor", json={"bucket_id": s.bucket(0.25)})
+    s.c.post("/requantize_weights", json={"format": "fp8_block"})
+    s.c.post("/update_weight_version", json={"new_version": 3})
+    s.c.post("/requantize_weights", json={"format": "mxfp8"})  # another format
+    assert s.seen == [0.5, 0.75, 0.25, 0.25, 0.25] and s.made == ["fp8_block", "fp8_block", "mxfp8"]
