@@ -587,14 +587,9 @@ class RLLoop:
 
     def _update_weights(self) -> dict:
         if getattr(self.args, "rollout_engine_urls", None):
-            out = self.weight_updater.update() if self.weight_updater is not None else {}
+            # --weight-sync-quant: the engines re-quantise what just arrived and serve from the block-scaled copies
             fmt = getattr(self.args, "weight_sync_quant", "none")
-            if fmt != "none" and self.ps.rank == 0:
-                # --weight-sync-quant: the engines re-quantise what just arrived and serve from the block-scaled copies
-                from .weight_sync.broadcast import HttpEngineHandle
-
-                for u in [x for x in self.args.rollout_engine_urls.split(",") if x]:
-                    HttpEngineHandle(u).post("/requantize_weights", {"format": fmt})
+            out = self.weight_updater.update(requantize=fmt) if self.weight_updater is not None else {}
             if self.ps.world_size > 1:
                 dist.barrier()  # nobody generates with the old weights while the first rank is still sending
             return out

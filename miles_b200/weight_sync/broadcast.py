@@ -7,7 +7,7 @@ trainer's source rank and every engine rank join a process group that exists onl
     pause_generation -> flush_cache -> for each bucket (<= buffer bytes):
         POST /update_weights_from_distributed {names, dtypes, shapes, group_name}     (engine starts receiving)
         broadcast(tensor, src=0) for every tensor of the bucket                        (trainer sends)
-    -> update_weight_version -> continue_generation
+    -> update_weight_version (-> requantize_weights) -> continue_generation
 
 Dense parameters go first, expert parameters second; under expert parallelism the source rank first gathers the
 experts of a bucket over the EP group so that engines see whole tensors.
@@ -202,7 +202,8 @@ class BroadcastWeightUpdater:
         yield dense
         yield experts
 
-    def update(self) -> dict:
+    def update(self, requantize: str = "none") -> dict:
+        """``requantize``: the block-scaled format that the engines serve from copies in; they make them of the new weights before they continue."""
         import time
 
         if not self.is_sender:
@@ -228,6 +229,8 @@ class BroadcastWeightUpdater:
                     h.result()
         for e in self.engines:
             e.post("/update_weight_version", {"new_version": version})
+            if requantize != "none":
+                e.post("/requantize_weights", {"format": requantize})
             e.post("/continue_generation", {})
         return {"perf/update_weights_time": time.perf_counter() - t0, "perf/update_weights_bytes": moved, "weight_version": version}
 

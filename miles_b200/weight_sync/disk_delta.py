@@ -137,7 +137,8 @@ class DiskDeltaUpdater:
         self.writer = DiskDeltaWriter(directory, encoding=encoding, checksum_kind=checksum_kind, rank=actor.ps.rank,
                                       world=actor.ps.world_size)
 
-    def update(self) -> dict:
+    def update(self, requantize: str = "none") -> dict:
+        """``requantize``: the block-scaled format that the engines serve from copies in."""
         import time
 
         import torch.distributed as dist
@@ -151,6 +152,9 @@ class DiskDeltaUpdater:
         futs = [h.post_async("/pull_weights", {"path": vdir, "weight_version": version}) for h in self.handles]
         for f in futs:
             f.result()
+        if requantize != "none":
+            for h in self.handles:
+                h.post("/requantize_weights", {"format": requantize})
         dt = time.perf_counter() - t0
         return {"perf/update_weights_time": dt, "perf/update_weights_total_time": dt, "perf/update_weights_bytes": idx["compressed_bytes"],
                 "perf/update_weights_raw_bytes": idx["raw_bytes"], "weight_version": version}
