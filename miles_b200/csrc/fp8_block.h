@@ -27,8 +27,9 @@ struct Fp8Gemm {
   void* workspace;    // fp8_gemm_workspace bytes, 16-byte aligned
 };
 long long fp8_gemm_workspace(const Fp8Gemm& p);
-// Launches of a product by expert: one, and one to join row tiles where the rows are many.
-int fp8_grouped_launches(long long rows, int groups);
+// Launches of a product by expert of `rows` rows with matrices [N, K] and a list of max_tiles row tiles: one, and one to join row tiles where pairs
+// of CTAs compute it.
+int fp8_grouped_launches(long long rows, int groups, int N, int K, bool gated, int max_tiles);
 // Launches on `stream`. Returns 0 or -1 with the reason in fp8_last_error().
 int fp8_gemm_launch(const Fp8Gemm& p, cudaStream_t stream);
 const char* fp8_last_error();

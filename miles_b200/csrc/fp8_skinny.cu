@@ -471,12 +471,17 @@ bool fp8_is_skinny(const Fp8Gemm& g) {
   return here <= there;
 }
 
-int fp8_grouped_launches(long long rows, int groups) {
+int fp8_grouped_launches(long long rows, int groups, int N, int K, bool gated, int max_tiles) {
+  if (rows <= 0 || max_tiles <= 0) return 0;
+  static uint8_t some[16];  // (which kernel it is does not depend on what lies where)
   Fp8Gemm g{};
   g.M = static_cast<int>(rows);
+  g.N = N;
+  g.K = K;
   g.groups = groups;
-  static const int some = 0;
-  g.tile_group = &some;
+  g.max_tiles = max_tiles;
+  g.tile_group = reinterpret_cast<const int*>(some);
+  if (gated) g.q = some;
   return fp8_is_skinny(g) ? 1 : 2;
 }
 

@@ -220,7 +220,7 @@ void register_fp8_block(pybind11::module_& m) {
   m.def("fp8_permute_rows", &fp8_permute_rows, py::arg("q"), py::arg("scales"), py::arg("src"), py::arg("num_tiles"), py::arg("top_k"));
   m.def("fp8_linear", &fp8_linear, py::arg("xq"), py::arg("xs"), py::arg("wq"), py::arg("ws"), py::arg("halves"), py::arg("residual") = py::none(),
         py::arg("tile_group") = py::none(), py::arg("num_tiles") = py::none(), py::arg("out") = py::none(), py::arg("status") = py::none());
-  m.def("fp8_grouped_launches", &mb::fp8_grouped_launches, py::arg("rows"), py::arg("experts"));
+  m.def("fp8_grouped_launches", &mb::fp8_grouped_launches, py::arg("rows"), py::arg("experts"), py::arg("n"), py::arg("k"), py::arg("gated"), py::arg("tiles"));
   m.def("fp8_gated_linear", &fp8_gated_linear, py::arg("xq"), py::arg("xs"), py::arg("wq"), py::arg("ws"), py::arg("halves"), py::arg("tile_group") = py::none(),
         py::arg("num_tiles") = py::none(), py::arg("status") = py::none());
 }

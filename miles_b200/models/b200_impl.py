@@ -422,7 +422,8 @@ class B200Qwen3:
             self.launches += 1
         act = F8.grouped_gated_linear(xp, w1_8, plan.tile_group, plan.num_tiles, self.status)
         yp = F8.grouped_linear(act, w2_8, plan.tile_group, plan.num_tiles, status=self.status)
-        self.launches += 2 * self.C.fp8_grouped_launches(plan.max_rows, w1_8.q.shape[0])
+        for w8 in (w1_8, w2_8):
+            self.launches += self.C.fp8_grouped_launches(plan.max_rows, *w8.q.shape, w8 is w1_8, plan.tile_group.shape[0])
         return yp
 
     def moe_forward(self, i, h2, replay_ids=None, record=None, keep=False, residual=None, serving=False, fp8=None):

@@ -76,7 +76,7 @@ def test_a_layer_is_computed_from_one_set_of_copies(preset, monkeypatch):
     model.attention = lambda q, k, v, cu: (torch.zeros(T, model.cfg.num_q_heads, model.cfg.head_dim, dtype=torch.bfloat16), None)
     model._route = lambda *a: (None, None, None)
     ids = torch.zeros(T, max(model.cfg.moe_top_k, 1), dtype=torch.int32)
-    model._permute_plan = lambda *a: type("Plan", (), dict(ids=ids, src=None, dest=None, tile_group=None, num_tiles=None, max_rows=ids.numel()))()
+    model._permute_plan = lambda *a: type("Plan", (), dict(ids=ids, src=None, dest=None, tile_group=ids, num_tiles=None, max_rows=ids.numel()))()
     model.layer_forward(0, torch.zeros(T, H, dtype=torch.bfloat16), None, None, T)
     assert [id(w) for w in read] == [id(w) for w in mine]
 
