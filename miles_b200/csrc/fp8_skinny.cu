@@ -369,7 +369,7 @@ int rows_of_tile(const Fp8Gemm& g) {
   if (!g.tile_group) return g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 || g.q ? 64 : 128;
   const long long live = g.groups < g.M ? g.groups : g.M;
   if (g.M <= 4 * live) return 16;
-  const long long rows = (g.M + g.M / 2) / live;
+  const long long rows = (static_cast<long long>(g.M) + g.M / 2) / live;
   return rows <= 32 ? 32 : rows <= 64 || g.q ? 64 : 128;
 }
 

@@ -37,7 +37,7 @@ void check_rows(const at::Tensor& q, const at::Tensor& s) {
   TORCH_CHECK(q.size(0) <= 1 || (q.stride(0) >= q.size(1) && q.stride(0) % 16 == 0), "x needs rows that are a multiple of 16 bytes apart");
   TORCH_CHECK(s.scalar_type() == at::kFloat && s.is_contiguous() && s.dim() == 2 && s.size(0) == q.size(0) && s.size(1) == blocks(q.size(1)),
               "x: scales must be contiguous fp32 [", q.size(0), ", ", blocks(q.size(1)), "]");
-  TORCH_CHECK(q.size(0) < (1ll << 31) - 128, "x: too many rows");
+  TORCH_CHECK(q.size(0) <= (1ll << 31) - 256, "x: at most 2^31 - 256 rows, which whole tiles of 256 reach in 32 bits, got ", q.size(0));
 }
 
 std::pair<at::Tensor, at::Tensor> new_rows(int64_t rows, int64_t cols, const at::Tensor& like) {
