@@ -22,8 +22,8 @@ void check_device(const at::Tensor& like, const at::Tensor& t, const char* name)
 void check_bf16_rows(const at::Tensor& t, int64_t rows, int64_t cols, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), name,
               " must be a bf16 matrix with contiguous rows");
-  TORCH_CHECK((rows < 0 || t.size(0) == rows) && (cols < 0 || t.size(1) == cols), name, " must be [", rows, ", ", cols, "], got [", t.size(0), ", ",
-              t.size(1), "]");
+  TORCH_CHECK((rows < 0 || t.size(0) == rows) && (cols < 0 || t.size(1) == cols), name, " must be a CUDA tensor [", rows, ", ", cols, "], got [",
+              t.size(0), ", ", t.size(1), "]");
   TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, ": rows must not overlap");
 }
 void check_vectors(const at::Tensor& t, const char* name) {
@@ -109,9 +109,9 @@ std::tuple<at::Tensor, at::Tensor> fp8_permute_rows(const at::Tensor& q, const a
   return {pq, ps};
 }
 
-// The parts of a product that all forms share: x, W [N, K] or [groups, N, K], and the row tiles of a grouped one.
+// The parts of a product: x, W [N, K] or [groups, N, K], the row tiles of a grouped one, and what an ungated one adds to and writes.
 mb::Fp8Gemm product(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor& wq, const at::Tensor& ws, bool gated, int64_t halves, const OptTensor& tile_group,
-                    const OptTensor& num_tiles, const OptTensor& status) {
+                    const OptTensor& num_tiles, const OptTensor& status, const OptTensor& residual = {}, const OptTensor& out = {}) {
   check_rows(xq, xs);
   const bool grouped = tile_group.has_value();
   TORCH_CHECK(grouped == num_tiles.has_value(), "tile_group and num_tiles are given together");
@@ -141,6 +141,8 @@ mb::Fp8Gemm product(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor
     TORCH_CHECK(tile_group->size(0) < (1 << 24), "tile_group: too many tiles");
   }
   if (status.has_value()) TORCH_CHECK(status->scalar_type() == at::kInt && status->numel() >= 1, "status must be int32");
+  if (residual.has_value()) check_bf16_rows(*residual, xq.size(0), N, "residual");
+  if (out.has_value()) check_bf16_rows(*out, xq.size(0), N, "out");
   check_device(xq, xq, "x");
   check_device(xq, xs, "x's scales");
   check_device(xq, wq, "weight");
@@ -158,6 +160,12 @@ mb::Fp8Gemm product(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor
     check_device(xq, *status, "status");
     p.status = status->data_ptr<int>();
   }
+  if (residual.has_value()) {
+    check_device(xq, *residual, "residual");
+    p.residual = residual->data_ptr();
+    p.ldr = pitch(*residual);
+  }
+  if (out.has_value()) check_device(xq, *out, "out");
   p.M = static_cast<int>(xq.size(0));
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
@@ -181,17 +189,7 @@ void launch(mb::Fp8Gemm& p, const at::Tensor& like, const char* name) {
 
 at::Tensor fp8_linear(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor& wq, const at::Tensor& ws, int64_t halves, const OptTensor& residual,
                       const OptTensor& tile_group, const OptTensor& num_tiles, const OptTensor& out, const OptTensor& status) {
-  mb::Fp8Gemm p = product(xq, xs, wq, ws, false, halves, tile_group, num_tiles, status);
-  if (residual.has_value()) {
-    check_bf16_rows(*residual, p.M, p.N, "residual");
-    check_device(xq, *residual, "residual");
-    p.residual = residual->data_ptr();
-    p.ldr = pitch(*residual);
-  }
-  if (out.has_value()) {
-    check_bf16_rows(*out, p.M, p.N, "out");
-    check_device(xq, *out, "out");
-  }
+  mb::Fp8Gemm p = product(xq, xs, wq, ws, false, halves, tile_group, num_tiles, status, residual, out);
   const c10::cuda::CUDAGuard guard(xq.device());
   at::Tensor y = out.has_value() ? *out : at::empty({p.M, p.N}, xs.options().dtype(at::kBFloat16));
   p.y = y.data_ptr();
