@@ -126,10 +126,19 @@ class RLLoop:
                                                                    + a.rollout_max_response_len + 8)
         page = getattr(a, "engine_page_size", 64)
         kv_bytes = None
+        pipelined = self.ps.pp.size > 1
+        sharded = getattr(self.actor, "fsdp", False)
+        quant = getattr(a, "rollout_quantization", "none") if self.actor.on_gpu and not self.actor.is_torch else "none"
+        copies = 0  # bytes of the block-scaled copies that the engine will serve from, beside its weights
+        if quant != "none":
+            from .models import build_specs
+
+            whole = pipelined or sharded or self.actor.ep_dispatcher is not None  # (the engine has a whole copy of the model, or may get one)
+            copies = self.actor.model.block_scaled_bytes(build_specs(cfg) if whole else self.actor.store.specs, quant)
         if self.actor.on_gpu:
             total = torch.cuda.get_device_properties(self.actor.device).total_memory
             frac = float(getattr(a, "sglang_mem_fraction_static", 0.7))
-            budget = int(total * frac) - self.actor.store.nbytes()
+            budget = int(total * frac) - self.actor.store.nbytes() - copies
             if getattr(self.actor, "fsdp", False):
                 budget -= sum(self.actor.store.full_sizes.values()) * 2  # the engine's own whole copy of the model
             per_tok = 2 * cfg.num_layers * cfg.num_kv_heads * cfg.head_dim * 2
@@ -141,11 +150,9 @@ class RLLoop:
             if getattr(a, "share_kv_grad_memory", True) and self.actor.store.grad.get("expert") is not None:
                 g = self.actor.store.grad["expert"]
                 lend = g.numel() * g.element_size()
-            room = free_now + lend - total // 7
+            room = free_now + lend - total // 7 - copies
             kv_bytes = max(min(budget, want, room), per_tok * page * 4)
-        pipelined = self.ps.pp.size > 1
-        sharded = getattr(self.actor, "fsdp", False)
-        replicate = not pipelined and self.actor.ep_dispatcher is not None and self._replicate_experts_fits(kv_bytes)
+        replicate = not pipelined and self.actor.ep_dispatcher is not None and self._replicate_experts_fits(kv_bytes, copies)
         if replicate:
             # the worst case (every sequence at the full context length) almost never happens and the engine retracts
             # requests when the pool runs dry: with the replica resident, size the pool for 65 % of that worst case
@@ -224,8 +231,7 @@ class RLLoop:
                 ep_decode = EpDecodeLL(cfg, self.ps, max_rows=max(max_running, 8))
             else:
                 ep_decode = ExpertParallel(cfg, self.ps, fused=one_node, max_tokens=max(max_running, 16))
-        quant = getattr(a, "rollout_quantization", "none")
-        if quant != "none" and self.actor.on_gpu and not self.actor.is_torch:
+        if quant != "none":
             if engine_model is self.actor.model:
                 # the trainer keeps multiplying bf16 weights: the engine gets a model object of its own on the same store
                 from .models import build_model
@@ -341,9 +347,9 @@ class RLLoop:
         moe_layers = sum(cfg.layer_is_moe(i) for i in range(cfg.num_layers))
         return moe_layers * cfg.num_experts * 3 * cfg.hidden_size * cfg.moe_ffn_hidden_size * 2
 
-    def _replicate_experts_fits(self, kv_bytes) -> bool:
+    def _replicate_experts_fits(self, kv_bytes, copies: int = 0) -> bool:
         """A full copy of the experts for the rollout engine, if asked for (default) and if it fits next to the
-        trainer's state, the KV cache and an activation reserve."""
+        trainer's state, the KV cache, the block-scaled copies of the weights and an activation reserve."""
         a = self.args
         from .trainer.actor import replica_wanted
 
@@ -353,7 +359,7 @@ class RLLoop:
         free_now, total = torch.cuda.mem_get_info(self.actor.device)
         g = self.actor.store.grad.get("expert")
         lend = g.numel() * g.element_size() if (g is not None and getattr(a, "share_kv_grad_memory", True)) else 0
-        need = replica + max((kv_bytes or 0) // 2 - lend, 0) + total // 7  # at least half of the wanted KV pool must remain
+        need = replica + copies + max((kv_bytes or 0) // 2 - lend, 0) + total // 7  # at least half of the wanted KV pool must remain
         ok = torch.tensor([1.0 if free_now >= need else 0.0], device=self.actor.device)
         if self.ps.world_size > 1:
             dist.all_reduce(ok, op=dist.ReduceOp.MIN)  # all ranks take the same path

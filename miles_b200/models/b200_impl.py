@@ -231,6 +231,18 @@ class B200Qwen3:
         self.mx = copies
         return len(copies)
 
+    @classmethod
+    def block_scaled_bytes(cls, specs, kind: str) -> int:
+        """What `enable_block_scaled` keeps for parameters of these names and shapes: values, and scales (twice for `csrc/gemm_mx.cu`, whose tensor
+        cores read them in another order)."""
+        n = 0
+        for s in specs:
+            if s.name.endswith(cls.MX_SUFFIXES):
+                rows, K = s.numel // s.shape[-1], s.shape[-1]
+                blocks = -(-rows // 128) * -(-K // 128)
+                n += {"none": 0, "mxfp8": s.numel + 2 * s.numel // 32, "nvfp4": s.numel // 2 + 2 * s.numel // 16, "fp8_block": s.numel + 4 * blocks}[kind]
+        return n
+
     @staticmethod
     def _quantize_mx(name, w, kind):
         from ..ops.mx_gemm import quantize_operand
