@@ -116,8 +116,8 @@ __global__ void fp8_block_kernel(const bf16* __restrict__ x, uint8_t* __restrict
                                  long long rows, long long cols, int ue8m0) {
   __shared__ float red[8];
   __shared__ float s_scale;
-  const long long br = blockIdx.y, bc = blockIdx.x;
-  const long long r0 = br * 128, c0 = bc * 128;
+  const unsigned blocks_c = static_cast<unsigned>((cols + 127) / 128);  // (blocks in one dimension: there can be more rows of them than a grid is high)
+  const long long r0 = static_cast<long long>(blockIdx.x / blocks_c) * 128, c0 = static_cast<long long>(blockIdx.x % blocks_c) * 128;
   float m = 0.f;
   for (int i = threadIdx.x; i < 128 * 128; i += blockDim.x) {
     const long long r = r0 + i / 128, c = c0 + i % 128;
@@ -132,7 +132,7 @@ __global__ void fp8_block_kernel(const bf16* __restrict__ x, uint8_t* __restrict
     float s = fmaxf(t, 1e-10f) / 448.f;
     if (ue8m0) s = e8m0_to_float(e8m0_ceil(s));
     s_scale = s;
-    sc[br * gridDim.x + bc] = s;
+    sc[blockIdx.x] = s;
   }
   __syncthreads();
   const float inv = 1.f / s_scale;
@@ -219,8 +219,8 @@ void absmax(const void* x, long long n, float* out, cudaStream_t s) {
 void quant_fp8_block128(const void* x, uint8_t* q, float* scales, long long rows, long long cols, bool ue8m0,
                         cudaStream_t s) {
   if (rows * cols <= 0) return;
-  dim3 grid(static_cast<unsigned>((cols + 127) / 128), static_cast<unsigned>((rows + 127) / 128));
-  fp8_block_kernel<<<grid, 256, 0, s>>>(static_cast<const bf16*>(x), q, scales, rows, cols, ue8m0 ? 1 : 0);
+  const long long blocks = ((cols + 127) / 128) * ((rows + 127) / 128);
+  fp8_block_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const bf16*>(x), q, scales, rows, cols, ue8m0 ? 1 : 0);
 }
 void fake_int4_quant(const void* x, void* y, void* scale, void* zero, long long rows, long long cols, int group_rows,
                      int group_cols, bool symmetric, cudaStream_t s) {
