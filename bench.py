@@ -119,7 +119,7 @@ def main() -> None:
     ap.add_argument("--max-tokens-per-gpu", type=int, default=32768)
     ap.add_argument("--no-routing-replay", action="store_true")
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel size (dense models; the rest of the GPUs are data parallel)")
-    ap.add_argument("--rollout-quantization", default="none", choices=["none", "mxfp8", "nvfp4"],
+    ap.add_argument("--rollout-quantization", default="none", choices=["none", "mxfp8", "nvfp4", "fp8_block"],
                     help="serve the rollout from block-scaled copies of the weights (not the headline configuration)")
     ap.add_argument("--pp", type=int, default=1, help="pipeline-parallel size (experts are then not expert parallel)")
     ap.add_argument("--budget-s", type=float, default=float(os.environ.get("BENCH_BUDGET_S", 760)),
