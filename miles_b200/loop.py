@@ -128,13 +128,9 @@ class RLLoop:
         kv_bytes = None
         pipelined = self.ps.pp.size > 1
         sharded = getattr(self.actor, "fsdp", False)
-        quant = getattr(a, "rollout_quantization", "none") if self.actor.on_gpu and not self.actor.is_torch else "none"
-        copies = 0  # bytes of the block-scaled copies that the engine will serve from, beside its weights
-        if quant != "none":
-            from .models import build_specs
+        from .trainer.actor import rollout_copy_bytes
 
-            whole = pipelined or sharded or self.actor.ep_dispatcher is not None  # (the engine has a whole copy of the model, or may get one)
-            copies = self.actor.model.block_scaled_bytes(build_specs(cfg) if whole else self.actor.store.specs, quant)
+        copies = rollout_copy_bytes(self.actor)
         if self.actor.on_gpu:
             total = torch.cuda.get_device_properties(self.actor.device).total_memory
             frac = float(getattr(a, "sglang_mem_fraction_static", 0.7))
@@ -231,7 +227,8 @@ class RLLoop:
                 ep_decode = EpDecodeLL(cfg, self.ps, max_rows=max(max_running, 8))
             else:
                 ep_decode = ExpertParallel(cfg, self.ps, fused=one_node, max_tokens=max(max_running, 16))
-        if quant != "none":
+        quant = getattr(a, "rollout_quantization", "none")
+        if quant != "none" and self.actor.on_gpu and not self.actor.is_torch:
             if engine_model is self.actor.model:
                 # the trainer keeps multiplying bf16 weights: the engine gets a model object of its own on the same store
                 from .models import build_model

@@ -45,7 +45,7 @@ def replica_wanted(args, ep_size: int) -> bool:
 
 def choose_memory_plan(total_bytes: int, dense_params: int, expert_params: int, reserve_frac: float = 0.16,
                        extra_resident_bytes: int = 0, kv_bytes: int = 0, dp_size: int = 1, state: str = "fp32",
-                       host_bytes: Optional[int] = None) -> dict:
+                       host_bytes: Optional[int] = None, copy_bytes: int = 0) -> dict:
     """Where the optimizer state of the expert group lives. The numerics do not depend on the placement:
     bf16 weights whose fp32 master is kept as (bf16 weight, signed 16-bit remainder), Adam moments in ``state``
     precision (fp32 like the reference's default optimizer, or bf16 like its precision-aware optimizer), fp32
@@ -55,7 +55,8 @@ def choose_memory_plan(total_bytes: int, dense_params: int, expert_params: int, 
     on the device and streams the rest through pinned host memory every optimizer step.
 
     ``reserve_frac`` of the device is left for activations, exchange buffers and the allocator;
-    ``extra_resident_bytes`` is whatever else will stay resident (e.g. a full expert replica for the engine);
+    ``extra_resident_bytes`` is whatever else will stay resident (e.g. a full expert replica for the engine); ``copy_bytes`` the
+    block-scaled copies that the engine is served from, which displace state as far as the host can take it (and the reserve beyond);
     ``kv_bytes`` the KV pool the engine will want (it shares the expert-gradient arena, so the larger of the two
     counts); the replicated parameters' state is partitioned over ``dp_size`` ranks; ``host_bytes`` is the pinned
     host memory this rank may take (None: unknown, not checked). Raises when device plus host cannot hold the state:
@@ -68,9 +69,11 @@ def choose_memory_plan(total_bytes: int, dense_params: int, expert_params: int, 
     room = int(total_bytes * (1.0 - reserve_frac)) - resident
     plan = dict(expert_grad="bf16", state=state, master=True, offload=False, resident_frac=1.0,
                 name=f"fp32 master, {state} moments")
-    if state_bytes > room:
-        frac = max(0.0, min(1.0, room / max(state_bytes, 1)))
-        frac = int(frac * 64) / 64.0  # whole chunks, rounded down
+    if state_bytes > room - copy_bytes:
+        chunks = lambda b: int(max(0.0, min(1.0, b / max(state_bytes, 1))) * 64)  # noqa: E731  (whole ones, rounded down)
+        frac = chunks(room - copy_bytes) / 64.0
+        if host_bytes is not None and copy_bytes:
+            frac = min(max(frac, 1.0 - chunks(host_bytes) / 64.0), max(frac, chunks(room) / 64.0))
         on_host = int(state_bytes * (1 - frac))
         if host_bytes is not None and on_host > host_bytes:
             raise MemoryError(
@@ -80,6 +83,19 @@ def choose_memory_plan(total_bytes: int, dense_params: int, expert_params: int, 
                 + (", or --use-precision-aware-optimizer --exp-avg-dtype bf16 --exp-avg-sq-dtype bf16" if state == "fp32" else ""))
         plan.update(offload=True, resident_frac=frac, name=plan["name"] + ", %d%% of the expert state streamed from host" % round(100 * (1 - frac)))
     return plan
+
+
+def rollout_copy_bytes(actor) -> int:
+    """Bytes of the block-scaled copies that the colocated engine will serve from beside its weights (``--rollout-quantization``)."""
+    quant = getattr(actor.args, "rollout_quantization", "none")
+    if quant == "none" or not actor.on_gpu or actor.is_torch:
+        return 0
+    from ..models import build_specs
+    from ..models.b200_impl import B200Qwen3
+
+    # (the engine of a pipelined or sharded trainer has a whole copy of the model, that of an expert-parallel one may get one)
+    whole = actor.ps.pp.size > 1 or actor.fsdp or actor.ps.ep.size > 1
+    return B200Qwen3.block_scaled_bytes(build_specs(actor.cfg) if whole else actor.store.specs, quant)
 
 
 def host_memory_per_rank(local_world: int) -> Optional[int]:
@@ -306,7 +322,7 @@ class TrainActor:
                 state = a.exp_avg_dtype if a.exp_avg_dtype in ("bf16", "fp32") else "bf16"
             local_world = int(os.environ.get("LOCAL_WORLD_SIZE", self.ps.world_size))
             plan = choose_memory_plan(total, dense, expert, extra_resident_bytes=extra, kv_bytes=kv, dp_size=self.ps.dp_cp.size,
-                                      state=state, host_bytes=host_memory_per_rank(local_world))
+                                      state=state, host_bytes=host_memory_per_rank(local_world), copy_bytes=rollout_copy_bytes(self) if colocated else 0)
         else:
             plan = dict(expert_grad="fp32", state="fp32", master=False, offload=False, resident_frac=1.0, name="cpu")
         if getattr(a, "main_params_dtype", "fp32") != "fp32":

@@ -94,3 +94,38 @@ def test_the_trainer_rolls_out_from_8_bit_copies(preset):
             kept = model.mx[w.data_ptr()]
             fresh = quantize_weight(w, kept.halves)
             assert torch.equal(kept.q.view(torch.uint8), fresh.q.view(torch.uint8)) and torch.equal(kept.scales, fresh.scales), name
+
+
+GB = 10 ** 9
+
+
+def plan(copies, host, total=190 * GB, experts=28 * GB):
+    from miles_b200.trainer.actor import choose_memory_plan
+
+    return choose_memory_plan(total, GB, experts, kv_bytes=0, state="bf16", host_bytes=host, copy_bytes=copies)
+
+
+def test_copies_displace_optimizer_state():
+    """190 GB, of which 84 % hold 12 of replicated parameters, 56 of expert weights and 56 of gradients: 35.6 are left for 168 of state, 13 of 64 chunks; with
+    30 of copies 2 of 64; and where the host takes 150, of the 168 at least 18: 7 of 64. Where the state without copies would have been placed it is placed."""
+    state = 6 * 28 * GB
+    assert plan(0, None)["resident_frac"] == plan(0, 200 * GB)["resident_frac"] == 13 / 64
+    assert plan(30 * GB, None)["resident_frac"] == plan(30 * GB, 200 * GB)["resident_frac"] == 2 / 64
+    tight = plan(30 * GB, 150 * GB)
+    assert tight["resident_frac"] == 7 / 64 and state * (1 - 7 / 64) <= 150 * GB < state * (1 - 6 / 64)
+    assert plan(30 * GB, int(state * (1 - 13 / 64)))["resident_frac"] == 13 / 64
+    for copies in (0, 30 * GB):  # what cannot be placed without copies cannot with them
+        with pytest.raises(MemoryError):
+            plan(copies, int(state * (1 - 13 / 64)) - GB)
+    assert plan(0, 0, total=400 * GB) == plan(30 * GB, 0, total=400 * GB) and not plan(0, 0, total=400 * GB)["offload"]
+
+
+@pytest.mark.gpu
+def test_the_optimizer_plan_is_told_of_the_copies(monkeypatch):
+    from miles_b200.trainer import actor
+
+    seen, ours = {}, actor.choose_memory_plan
+    for kind in ("none", "fp8_block"):
+        monkeypatch.setattr(actor, "choose_memory_plan", lambda *a, **k: seen.setdefault(kind, k["copy_bytes"]) and None or ours(*a, **k))
+        loop("qwen3-smoke", kind)
+    assert seen["none"] == 0 and abs(seen["fp8_block"] - held_by("fp8_block")) <= 1024
