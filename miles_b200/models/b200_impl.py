@@ -203,10 +203,9 @@ class B200Qwen3:
     def enable_block_scaled(self, kind: str) -> int:
         """Serve the projections and experts from MXFP8 / NVFP4 copies of the weights (`csrc/gemm_mx.cu`) whenever
         more than 32 rows are multiplied, or from E4M3 copies with a scale for each 128 x 128 (``fp8_block``, `ops/fp8_block.py`) whenever more
-        than ``SMALL_T`` are; the few-row decode kernels keep streaming the bf16 weights. Meant for a
-        model object that only the rollout engine uses. Experts of an expert-parallel model stay in bf16. Call again (or `refresh_block_scaled`) after a weight update: copies
-        of the same format are written where they are, since captured decode steps read them there.
-        Returns the number of tensors quantised."""
+        than ``SMALL_T`` are; the few-row decode kernels keep streaming the bf16 weights, and the experts of an expert-parallel model stay in
+        bf16. Meant for a model object that only the rollout engine uses. Call again (or `refresh_block_scaled`) after a weight update: copies of the
+        same format are written where they are, since captured decode steps read them there. Returns the number of tensors quantised."""
         if kind not in ("mxfp8", "nvfp4", "fp8_block"):
             raise ValueError(f"unknown block-scaled kind {kind!r}")
         quantize = self._quantize_fp8_block if kind == "fp8_block" else self._quantize_mx
