@@ -24,8 +24,8 @@
 // operands; with stores by threads, from half of that: 87 -> 73 us at 32768 x 2048 x 768, 129 -> 118 at K = 1536, 146 -> 143 at 8192 x 2048 x
 // 8192). An expert's last rows, with another's behind them in the box, and rows of y that do not begin or end at 16 bytes are stored by threads.
 //
-// Measured, us: 8192 x 24576 x 4096 gate-up 942 (1750 TFLOP/s), 8192 x 4096 x 4096 with residual 142, experts of 65536 rows, 128 of 1536 x
-// 2048 gate-up 341, 2048 x 768 199.
+// Measured, us: 8192 x 24576 x 4096 gate-up 942 (1750 TFLOP/s), 8192 x 4096 x 4096 with residual 142 (160 in a long run, at the clock that its
+// power leaves), experts of 65536 rows, 128 of 1536 x 2048 gate-up 341, 2048 x 768 199.
 //
 // Reference counterpart: the block-wise FP8 GEMMs of the serving engines that load its FP8 checkpoints (weight_block_size [128, 128]:
 // miles/backends/megatron_utils/megatron_to_hf/processors/quantizer_fp8.py, miles/utils/fp8_kernel.py:24-79).

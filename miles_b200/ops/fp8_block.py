@@ -7,11 +7,12 @@ one fp32 scale for each 128 x 128 (`weight_sync.quantize`, format ``fp8_block``)
 * `linear` and `grouped_linear` multiply them with a weight, or by expert over row tiles: bf16 results;
 * `gated_linear` and `grouped_gated_linear` multiply them with a gate-up weight and leave ``silu(gate) * up`` as 8-bit rows again.
 
-Rows are a multiple of 16 wide; nothing else about the sizes has to be even, rows of `x` may be apart, and no rows are fine. Row tiles are those
-of the router's sort (``moe_build_permutation``): int32 ``{expert, first row, rows (at most 128), 0}`` of which the first ``num_tiles[0]``
+Rows are a multiple of 16 wide, and at most 2^31 - 256; nothing else about the sizes has to be even, rows of `x` may be apart, and no rows are
+fine. Row tiles are those of the router's sort (``moe_build_permutation``): int32 ``{expert, first row, rows (at most 128), 0}`` of which the first ``num_tiles[0]``
 are live; each row of the result belongs to at most one tile, and rows that belong to none are left unwritten. A block that holds NaN or
-an infinity gets that scale, and what is multiplied with it becomes NaN. Everything runs on the current stream without a
-workspace or a wait of the host, so it can be captured. Inference only: weights that are trained stay in bf16.
+an infinity gets that scale, and what is multiplied with it becomes NaN. Everything runs on the current stream without a wait of the host, and the
+list of joined row tiles that products by expert of many rows need is the allocator's, so calls can be captured and run beside one another.
+Inference only: weights that are trained stay in bf16.
 
 ``status`` is the models' device status word: it receives a code should a wait inside a kernel ever run out.
 
@@ -99,7 +100,8 @@ def _rows(x: Union[Fp8Rows, torch.Tensor]) -> Fp8Rows:
 
 def linear(x: Union[Fp8Rows, torch.Tensor], w: Fp8Weight, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x @ w^T (+ residual)`` in bf16, rounded once; ``x`` as 8-bit rows, or in bf16 (quantised first). ``out`` may be the residual itself."""
+    """``x @ w^T (+ residual)`` in bf16, rounded once; ``x`` as 8-bit rows, or in bf16 (quantised first). ``out`` may be the residual itself,
+    and shares no memory with the operands otherwise."""
     x = _rows(x)
     return _ext.load(required=True).fp8_linear(x.q, x.scales, w.q, w.scales, w.halves, residual, None, None, out, status)
 
